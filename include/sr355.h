@@ -37,6 +37,7 @@ extern "C" {
 
 #define SR355_DTYPE_BF16 0       /* bf16 storage, fp32 accumulate (32x32x16 MFMA) */
 #define SR355_DTYPE_F32 1        /* fp32 storage, exact fp32 MFMA (32x32x2)        */
+#define SR355_DTYPE_F16 2        /* fp16 storage: the operators on rows of channels only */
 
 /* Split modes (bf16 only).  A bf16 product keeps 8 significant bits per factor; where that is
  * not enough the rounding residue is carried as extra terms of the same MFMA accumulation:
@@ -51,7 +52,7 @@ extern "C" {
 #define SR355_PACK_F16 3    /* sr355_pack_weight only (bf16 dtype): one weight image stored as IEEE fp16, for a
                               conv run with f16_in = 1 */
 
-#define SR355_ABI_VERSION 18
+#define SR355_ABI_VERSION 19
 
 int sr355_abi_version(void);
 const char *sr355_last_error(void);
@@ -342,6 +343,61 @@ int sr355_maxpool2x2_bwd(const void *in_act_dev, size_t in_bytes, const void *dy
 size_t sr355_loss_workspace_bytes(size_t n);
 int sr355_loss_fwd(const float *a_dev, const float *b_dev, float b_const, size_t n, int mode, float *loss_dev,
                    float *grad_dev, void *workspace_dev, size_t workspace_bytes, void *stream);
+
+/* ---- operators on rows of channels ("tokens": an image's pixels, one row of `channels` elements each) ----
+ * No counterpart in the reference, whose blocks normalise per channel (nn.BatchNorm2d, esrgan_model.py:68-72) and mix
+ * channels in 3x3 convs (:10-24): the channel-mixing half of a residual block with layer normalisation, a gated
+ * feed-forward block and dropout onto the skip.  Tensors are row-major with `channels` contiguous; a row stride (`*_ld`)
+ * is given in elements where an input may be a view.  dtype SR355_DTYPE_BF16, _F16 or _F32; sums and statistics are fp32
+ * and of a fixed order.  Any sizes, strides and alignment are taken; widths, strides and pointers that are multiples of 16
+ * bytes run on 16-byte accesses. */
+
+/* y = (x - mean) / sqrt(var + eps) * w + b over the C channels of each row.  w and b may be null; they are of the
+ * activations' type or fp32 (w_dtype).  mean / rstd [rows] fp32 for the backward pass (both null: not written). */
+int sr355_layer_norm_fwd(const void *x_dev, long long rows, int C, long long x_ld, int dtype, const void *w_dev,
+                         const void *b_dev, int w_dtype, float eps, void *y_dev, float *mean_dev, float *rstd_dev,
+                         void *stream);
+/* dx [rows][C], dw and db [C] of w_dtype; each may be null.  The workspace is needed for dw / db only. */
+size_t sr355_layer_norm_bwd_workspace_bytes(int C);
+int sr355_layer_norm_bwd(const void *dy_dev, long long dy_ld, const void *x_dev, long long x_ld, long long rows, int C,
+                         int dtype, const void *w_dev, int w_dtype, const float *mean_dev, const float *rstd_dev,
+                         void *dx_dev, void *dw_dev, void *db_dev, void *workspace_dev, size_t workspace_bytes,
+                         void *stream);
+
+/* y = (keep ? x / (1 - p) : 0) + skip over n contiguous elements (skip may be null); the gradient of x is the same call
+ * on the gradient of y, without a skip.  Element i is kept by 16 bits of Philox 4x32 with 7 rounds, key rng[0], counter
+ * (i / 8, rng[1] mod 2^32, site); p counts in steps of 2^-16.  rng: two 64-bit words in device memory. */
+int sr355_dropout(const void *x_dev, const void *skip_dev, long long n, int dtype, double p, const long long *rng_dev,
+                  unsigned site, void *y_dev, void *stream);
+
+/* Gated feed-forward block: y = (act(x Wg' + bg) * (x Wu' + bu)) Wd' + bd. */
+#define SR355_ACT_SILU 0
+#define SR355_ACT_GELU 1    /* g * Phi(g), by erf */
+#define SR355_ACT_RELU 2
+#define SR355_ACT_SIGMOID 3
+typedef struct sr355_ffn_args {
+    int dtype, activation;     /* SR355_DTYPE_*, SR355_ACT_*                                        */
+    long long rows;
+    int channels, hidden;
+    const void *x_dev;         /* [rows][channels], row stride x_ld                                 */
+    long long x_ld;
+    const void *w_gate_dev, *w_up_dev;   /* [hidden][channels]                                       */
+    const void *w_down_dev;              /* [channels][hidden]                                       */
+    const void *b_gate_dev, *b_up_dev, *b_down_dev;   /* may be null                                 */
+    void *y_dev;               /* forward: [rows][channels]                                         */
+    void *saved_dev;           /* forward: written where not null; backward: read                   */
+    size_t saved_bytes;        /* sr355_gated_ffn_saved_bytes                                       */
+    const void *dy_dev;        /* backward: gradient of y, row stride dy_ld                         */
+    long long dy_ld;
+    /* backward: any of these may be null (not computed)                                            */
+    void *dx_dev, *dw_gate_dev, *dw_up_dev, *dw_down_dev, *db_gate_dev, *db_up_dev, *db_down_dev;
+    void *workspace_dev;       /* sr355_gated_ffn_workspace_bytes of the same arguments             */
+    size_t workspace_bytes;
+} sr355_ffn_args;
+size_t sr355_gated_ffn_saved_bytes(const sr355_ffn_args *args);
+size_t sr355_gated_ffn_workspace_bytes(const sr355_ffn_args *args, int backward);
+int sr355_gated_ffn_fwd(const sr355_ffn_args *args, void *stream);
+int sr355_gated_ffn_bwd(const sr355_ffn_args *args, void *stream);
 
 /* ---- whole generator (GeneratorRRDB.forward, esrgan_model.py:55-62) ---- */
 typedef struct sr355_generator_cfg {

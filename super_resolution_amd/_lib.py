@@ -16,7 +16,8 @@ CSRC_DIR = os.path.join(_HERE, "csrc")
 
 DTYPE_BF16 = 0
 DTYPE_F32 = 1
-ABI_VERSION = 18
+DTYPE_F16 = 2   # the operators on rows of channels only
+ABI_VERSION = 19
 SPLIT_NONE, SPLIT_WEIGHT, SPLIT_INPUT = 0, 1, 2
 STATIC_SCRATCH_BYTES = 16 << 20   # SR355_STATIC_SCRATCH_BYTES
 PACK_F16 = 3     # sr355_pack_weight: one weight image stored as fp16
@@ -43,6 +44,8 @@ EXPORTS = (
     "sr355_bn_workspace_bytes", "sr355_bn_lrelu_fwd", "sr355_bn_lrelu_bwd", "sr355_bn_lrelu_fwd_groups",
     "sr355_bn_lrelu_bwd_groups",
     "sr355_pixel_shuffle2", "sr355_maxpool2x2_fwd", "sr355_maxpool2x2_bwd", "sr355_loss_workspace_bytes", "sr355_loss_fwd",
+    "sr355_layer_norm_fwd", "sr355_layer_norm_bwd_workspace_bytes", "sr355_layer_norm_bwd", "sr355_dropout",
+    "sr355_gated_ffn_saved_bytes", "sr355_gated_ffn_workspace_bytes", "sr355_gated_ffn_fwd", "sr355_gated_ffn_bwd",
 )
 
 
@@ -125,6 +128,21 @@ class DenseWgradArgs(C.Structure):
         ("units", C.c_int), ("num_features", C.c_int), ("growth_channels", C.c_int),
         ("growth_scale", C.c_float), ("conv5_scale", C.c_float),
         ("dw_dev", C.c_void_p * 5), ("db_dev", C.c_void_p * 5),
+        ("workspace_dev", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
+class FfnArgs(C.Structure):
+    """Mirror of ``sr355_ffn_args``."""
+    _fields_ = [
+        ("dtype", C.c_int), ("activation", C.c_int), ("rows", C.c_longlong), ("channels", C.c_int), ("hidden", C.c_int),
+        ("x_dev", C.c_void_p), ("x_ld", C.c_longlong),
+        ("w_gate_dev", C.c_void_p), ("w_up_dev", C.c_void_p), ("w_down_dev", C.c_void_p),
+        ("b_gate_dev", C.c_void_p), ("b_up_dev", C.c_void_p), ("b_down_dev", C.c_void_p),
+        ("y_dev", C.c_void_p), ("saved_dev", C.c_void_p), ("saved_bytes", C.c_size_t),
+        ("dy_dev", C.c_void_p), ("dy_ld", C.c_longlong),
+        ("dx_dev", C.c_void_p), ("dw_gate_dev", C.c_void_p), ("dw_up_dev", C.c_void_p), ("dw_down_dev", C.c_void_p),
+        ("db_gate_dev", C.c_void_p), ("db_up_dev", C.c_void_p), ("db_down_dev", C.c_void_p),
         ("workspace_dev", C.c_void_p), ("workspace_bytes", C.c_size_t),
     ]
 
@@ -233,6 +251,19 @@ def lib() -> C.CDLL:
     L.sr355_loss_workspace_bytes.argtypes = [sz]
     L.sr355_loss_workspace_bytes.restype = sz
     L.sr355_loss_fwd.argtypes = [vp, vp, f, sz, i, vp, vp, vp, sz, vp]
+    ll = C.c_longlong
+    L.sr355_layer_norm_fwd.argtypes = [vp, ll, i, ll, i, vp, vp, i, f, vp, vp, vp, vp]
+    L.sr355_layer_norm_bwd_workspace_bytes.argtypes = [i]
+    L.sr355_layer_norm_bwd_workspace_bytes.restype = sz
+    L.sr355_layer_norm_bwd.argtypes = [vp, ll, vp, ll, ll, i, i, vp, i, vp, vp, vp, vp, vp, vp, sz, vp]
+    L.sr355_dropout.argtypes = [vp, vp, ll, i, C.c_double, vp, C.c_uint, vp, vp]
+    ffnp = C.POINTER(FfnArgs)
+    L.sr355_gated_ffn_saved_bytes.argtypes = [ffnp]
+    L.sr355_gated_ffn_saved_bytes.restype = sz
+    L.sr355_gated_ffn_workspace_bytes.argtypes = [ffnp, i]
+    L.sr355_gated_ffn_workspace_bytes.restype = sz
+    L.sr355_gated_ffn_fwd.argtypes = [ffnp, vp]
+    L.sr355_gated_ffn_bwd.argtypes = [ffnp, vp]
     if L.sr355_abi_version() != ABI_VERSION:
         raise Sr355Error(f"libsr355.so ABI {L.sr355_abi_version()} != expected {ABI_VERSION}; rebuild")
     _lib = L

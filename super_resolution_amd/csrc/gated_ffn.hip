@@ -1,0 +1,463 @@
+// The gated feed-forward block on rows of channels and its gradients:
+//     g = x Wg' + bg, u = x Wu' + bu, h = act(g) * u, y = h Wd' + bd;
+//     dh = dy Wd, dg = dh * u * act'(g), du = dh * act(g), dx = dg Wg + du Wu,
+//     dWg = dg' x, dWu = du' x, dWd = dy' h, biases: column sums of dg, du, dy.
+// Forward: one launch computes both projections, the activation and the product (a workgroup multiplies its rows of x with
+// the gate and the up weights of the same hidden channels, so g and u meet in a wave's registers), one the projection back.
+// Backward: one launch computes dh and, in its epilogue, dg and du; one dx over both sections of k; one all three weight
+// gradients.  Products accumulate in fp32.  Between the launches g, u, h, dg and du are held in the type of x: as products'
+// operands they are rounded to it in any case, and g and u kept in fp32 would double the traffic of the two launches that
+// are nearest to the memory's pace.  Training keeps g, u and h (three rows of hidden channels each); inference h alone.
+//
+// Operands are read 16 bytes at a time.  What does not allow that (a width, stride or pointer that is no multiple of 16
+// bytes) is first copied into padded rows of the workspace, one launch for all of them.
+#include "token_gemm.h"
+
+namespace sr355 {
+
+namespace {
+// tiles: 256 x 256 with eight waves where that fills the chip, else 128 x 128 with four waves, two workgroups per CU
+typedef TokTile<256, 256, 2, 4, 2> Tile256;
+typedef TokTile<128, 128, 2, 2, 2> Tile128;
+constexpr int N_CU = 256;
+
+struct PadJob {
+    const void *src;
+    void *dst;
+    long long rows, src_ld, dst_ld;   // elements
+    int cols;
+};
+struct PadArgs {
+    PadJob job[5];
+};
+// rows of `cols` elements into rows of dst_ld (a multiple of a unit), zeros behind
+template <typename T>
+__global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs p) {
+    constexpr int E = 16 / sizeof(T);
+    const PadJob &j = p.job[blockIdx.y];
+    const long long units = j.dst_ld / E, n = j.rows * units;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+        const long long row = i / units;
+        const int c = (int)(i - row * units) * E;
+        const T *src = (const T *)j.src + row * j.src_ld + c;
+        TokUnit<T> u;
+#pragma unroll
+        for (int e = 0; e < E; ++e) u.v[e] = c + e < j.cols ? src[e] : (T)0.f;
+        tok_store_unit((T *)j.dst + i * E, u);
+    }
+}
+
+// out[j] = sum over splits, in order, of part[s * n + j]
+struct ReduceArgs {
+    const float *part[3];
+    void *out[3];
+    long long n[3];
+    int splits;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void reduce_splits_kernel(ReduceArgs a) {
+    const float *part = a.part[blockIdx.y];
+    T *out = (T *)a.out[blockIdx.y];
+    const long long n = a.n[blockIdx.y];
+    const bool vec = (n & 3) == 0 && ((size_t)out & 15) == 0;
+    for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (long long)gridDim.x * 1024) {
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (vec) {
+            for (int s = 0; s < a.splits; ++s) {
+                float t[4];
+                tok_load4<float>(part + (size_t)s * n + i, t);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] += t[j];
+            }
+            tok_store4<T>(out + i, v);
+        } else {
+            for (int j = 0; j < 4 && i + j < n; ++j) {
+                for (int s = 0; s < a.splits; ++s) v[j] += part[(size_t)s * n + i + j];
+                out[i + j] = (T)v[j];
+            }
+        }
+    }
+}
+
+// Column sums of up to three matrices of rows (16-byte rows): workgroup (part, block of 32 units, matrix), thread
+// (unit, one of 8 row groups); the row groups meet in the LDS.
+struct ColJob {
+    const void *src;
+    long long ld, first;     // first: column of the job in a partial row
+    int cols;
+};
+struct ColArgs {
+    ColJob job[3];
+    float *parts;
+    long long rows, stride;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void column_sums_kernel(ColArgs a) {
+    constexpr int E = 16 / sizeof(T);
+    __shared__ float red[8][32 * E + 1];
+    const ColJob &j = a.job[blockIdx.z];
+    const int ul = threadIdx.x & 31, rg = threadIdx.x >> 5;
+    const int c = (blockIdx.y * 32 + ul) * E;
+    float s[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) s[e] = 0.f;
+    if (c < j.cols) {
+        for (long long r = (long long)blockIdx.x * 8 + rg; r < a.rows; r += (long long)gridDim.x * 8) {
+            float v[E];
+            tok_load<T, E>((const T *)j.src + r * j.ld + c, v);
+#pragma unroll
+            for (int e = 0; e < E; ++e) s[e] += v[e];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) red[rg][ul * E + e] = s[e];
+    __syncthreads();
+    for (int k = threadIdx.x; k < 32 * E; k += 256) {
+        const int col = blockIdx.y * 32 * E + k;
+        if (col >= j.cols) continue;
+        float t = 0.f;
+        for (int r = 0; r < 8; ++r) t += red[r][k];
+        a.parts[(size_t)blockIdx.x * a.stride + j.first + col] = t;
+    }
+}
+constexpr int COL_PARTS = 128;
+
+template <typename T, typename G, bool A_RC, bool B_RC, int EPI>
+int gemm_launch(const TokGemmArgs &g, const char *what, hipStream_t stream) {
+    void (*const kernel)(TokGemmArgs) = tok_gemm_kernel<T, G, A_RC, B_RC, EPI>;
+    if (G::LDS_BYTES > 64 * 1024) {
+        // (per device, and cheap: not remembered)
+        const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS_BYTES);
+        if (e != hipSuccess) return check_hip(e, what);
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(g.n_tiles * g.splits)), dim3(G::THREADS), G::LDS_BYTES, stream, g);
+    return check_hip(hipGetLastError(), what);
+}
+
+template <typename G>
+long long set_tiles(TokGemmArgs &g, bool glu) {
+    long long n = 0;
+    for (int j = 0; j < g.n_jobs; ++j) {
+        g.first_tile[j] = (int)n;
+        g.job[j].tiles_m = (int)tok_cdiv(g.job[j].M, G::BM);
+        g.job[j].tiles_n = (int)tok_cdiv(g.job[j].N, glu ? G::BN / 2 : G::BN);
+        n += (long long)g.job[j].tiles_m * g.job[j].tiles_n;
+    }
+    g.n_tiles = (int)n;
+    return n;
+}
+
+template <typename T, bool A_RC, bool B_RC, int EPI>
+int gemm_pick(TokGemmArgs &g, const char *what, hipStream_t stream) {
+    g.splits = 1;
+    const bool glu = EPI == TOK_EPI_GLU;
+    if (set_tiles<Tile256>(g, glu) >= N_CU) return gemm_launch<T, Tile256, A_RC, B_RC, EPI>(g, what, stream);
+    if (set_tiles<Tile128>(g, glu) > 0x3fffffffLL) {
+        set_error("%s: too many tiles", what);
+        return SR355_ERR_INVALID;
+    }
+    return gemm_launch<T, Tile128, A_RC, B_RC, EPI>(g, what, stream);
+}
+
+// ---- the plan of a call: what is copied, where things lie in the workspace --------------------------------------------
+struct Operand {
+    const void *p;
+    long long ld;     // elements
+};
+struct Plan {
+    size_t at = 0;
+    unsigned char *base = nullptr;
+    PadArgs pads;
+    int n_pads = 0;
+
+    void *take(size_t bytes) {
+        void *r = base ? base + at : nullptr;
+        at += (bytes + 255) & ~(size_t)255;
+        return r;
+    }
+    // the operand as it is where 16-byte reads can have it, else its padded copy
+    Operand operand(const void *p, long long rows, int cols, long long ld, int dtype) {
+        const int e = dtype == SR355_DTYPE_F32 ? 4 : 8;
+        const long long row_bytes = ld * (long long)tok_type_bytes(dtype);
+        if (cols % e == 0 && ld % e == 0 && tok_aligned16(p) && row_bytes < (1LL << 22)) return {p, ld};
+        const long long dst_ld = round_up(cols, e);
+        void *dst = take((size_t)rows * dst_ld * tok_type_bytes(dtype));
+        pads.job[n_pads++] = {p, dst, rows, ld, dst_ld, cols};
+        return {dst, dst_ld};
+    }
+};
+
+template <typename T>
+int run_pads(const Plan &plan, hipStream_t stream) {
+    if (!plan.n_pads) return SR355_OK;
+    long long most = 0;
+    for (int i = 0; i < plan.n_pads; ++i) {
+        const long long n = plan.pads.job[i].rows * plan.pads.job[i].dst_ld * (long long)sizeof(T) / 16;
+        if (n > most) most = n;
+    }
+    if (most == 0) return SR355_OK;
+    const long long wgs = tok_cdiv(most, 256);
+    hipLaunchKernelGGL((pad_rows_kernel<T>), dim3((unsigned)(wgs > 4096 ? 4096 : wgs), plan.n_pads), dim3(256), 0, stream, plan.pads);
+    return check_hip(hipGetLastError(), "gated_ffn row padding launch");
+}
+
+long long hidden_ld(const sr355_ffn_args *a) { return round_up(a->hidden, a->dtype == SR355_DTYPE_F32 ? 4 : 8); }
+
+size_t hidden_bytes(const sr355_ffn_args *a) {
+    return ((size_t)a->rows * hidden_ld(a) * tok_type_bytes(a->dtype) + 255) & ~(size_t)255;
+}
+
+struct ForwardPlan : Plan {
+    Operand x, wg, wu, wd;
+    void *g, *u, *h;
+
+    ForwardPlan(const sr355_ffn_args *a, unsigned char *ws) {
+        base = ws;
+        x = operand(a->x_dev, a->rows, a->channels, a->x_ld, a->dtype);
+        wg = operand(a->w_gate_dev, a->hidden, a->channels, a->channels, a->dtype);
+        wu = operand(a->w_up_dev, a->hidden, a->channels, a->channels, a->dtype);
+        wd = operand(a->w_down_dev, a->channels, a->hidden, a->hidden, a->dtype);
+        if (a->saved_dev) {
+            unsigned char *s = (unsigned char *)a->saved_dev;
+            g = s, u = s + hidden_bytes(a), h = s + 2 * hidden_bytes(a);
+        } else {
+            g = u = nullptr, h = take(hidden_bytes(a));
+        }
+    }
+};
+
+// Workgroups of the weight gradients: k is the rows, so a few tiles with a long k are split until the chip is full, with
+// at least eight stages (512 rows) a split.
+struct WgradShape {
+    bool big;
+    int splits, split_stages;
+};
+template <typename G>
+long long wgrad_tiles(const sr355_ffn_args *a) {
+    const long long f_c = tok_cdiv(a->hidden, G::BM) * tok_cdiv(a->channels, G::BN);
+    const long long c_f = tok_cdiv(a->channels, G::BM) * tok_cdiv(a->hidden, G::BN);
+    return (a->dw_gate_dev ? f_c : 0) + (a->dw_up_dev ? f_c : 0) + (a->dw_down_dev ? c_f : 0);
+}
+WgradShape wgrad_shape(const sr355_ffn_args *a) {
+    const long long stages = tok_cdiv(a->rows, 128 / (long long)tok_type_bytes(a->dtype));
+    WgradShape w;
+    w.big = wgrad_tiles<Tile256>(a) >= N_CU / 4;
+    const long long tiles = w.big ? wgrad_tiles<Tile256>(a) : wgrad_tiles<Tile128>(a);
+    const long long want = tok_cdiv(w.big ? N_CU : 2 * N_CU, tiles < 1 ? 1 : tiles);
+    long long splits = stages / 8 < want ? stages / 8 : want;
+    if (splits < 1) splits = 1;
+    w.split_stages = (int)tok_cdiv(stages < 1 ? 1 : stages, splits);
+    w.splits = (int)tok_cdiv(stages < 1 ? 1 : stages, w.split_stages);
+    return w;
+}
+
+struct BackwardPlan : Plan {
+    Operand x, dy, wg, wu, wd;
+    void *dg, *du;
+    const void *g, *u, *h;
+    float *parts, *col_parts;
+    WgradShape wgrad;
+    bool need_hidden;
+
+    BackwardPlan(const sr355_ffn_args *a, unsigned char *ws) {
+        base = ws;
+        const bool gate_up = a->dw_gate_dev || a->dw_up_dev;
+        need_hidden = a->dx_dev || gate_up || a->db_gate_dev || a->db_up_dev;
+        x = wg = wu = wd = {nullptr, 0};
+        dy = operand(a->dy_dev, a->rows, a->channels, a->dy_ld, a->dtype);
+        if (gate_up) x = operand(a->x_dev, a->rows, a->channels, a->x_ld, a->dtype);
+        if (a->dx_dev) {
+            wg = operand(a->w_gate_dev, a->hidden, a->channels, a->channels, a->dtype);
+            wu = operand(a->w_up_dev, a->hidden, a->channels, a->channels, a->dtype);
+        }
+        if (need_hidden) wd = operand(a->w_down_dev, a->channels, a->hidden, a->hidden, a->dtype);
+        const unsigned char *s = (const unsigned char *)a->saved_dev;
+        g = s, u = s + hidden_bytes(a), h = s + 2 * hidden_bytes(a);
+        dg = need_hidden ? take(hidden_bytes(a)) : nullptr;
+        du = need_hidden ? take(hidden_bytes(a)) : nullptr;
+        wgrad = wgrad_shape(a);
+        const size_t mats = (a->dw_gate_dev != nullptr) + (a->dw_up_dev != nullptr) + (a->dw_down_dev != nullptr);
+        parts = mats && wgrad.splits > 1
+                    ? (float *)take(mats * wgrad.splits * (size_t)a->hidden * a->channels * sizeof(float)) : nullptr;
+        const bool cols = a->db_gate_dev || a->db_up_dev || a->db_down_dev;
+        col_parts = cols ? (float *)take((size_t)COL_PARTS * (2 * hidden_ld(a) + dy.ld) * sizeof(float)) : nullptr;
+    }
+};
+
+bool ffn_args_ok(const char *who, const sr355_ffn_args *a, bool backward) {
+    if (!a || !tok_dtype_ok(a->dtype) || a->activation < 0 || a->activation > SR355_ACT_SIGMOID || a->rows < 0 ||
+        a->rows > 0x7fffff00LL || a->channels < 1 || a->hidden < 1 || a->channels > (1 << 20) || a->hidden > (1 << 20) ||
+        a->x_ld < a->channels || (backward && a->dy_ld < a->channels)) {
+        if (!a) set_error("%s: null arguments", who);
+        else
+            set_error("%s: bad arguments (dtype=%d activation=%d rows=%lld channels=%d hidden=%d, row strides %lld and %lld; "
+                      "widths up to 2^20, fewer than 2^31 rows)", who, a->dtype, a->activation, a->rows, a->channels, a->hidden,
+                      a->x_ld, a->dy_ld);
+        return false;
+    }
+    return true;
+}
+
+template <typename T>
+int ffn_forward(const sr355_ffn_args *a, hipStream_t stream) {
+    ForwardPlan p(a, (unsigned char *)a->workspace_dev);
+    int rc = run_pads<T>(p, stream);
+    if (rc != SR355_OK) return rc;
+    TokGemmArgs g = {};
+    g.n_jobs = 1, g.sections = 1, g.act = a->activation, g.K = a->channels;
+    TokJob &j = g.job[0];
+    j.a[0] = (const unsigned char *)p.x.p, j.a_ld = p.x.ld * sizeof(T);
+    j.b[0] = (const unsigned char *)p.wg.p, j.b[1] = (const unsigned char *)p.wu.p, j.b_ld = p.wg.ld * sizeof(T);
+    j.M = (int)a->rows, j.N = a->hidden, j.bias = a->b_gate_dev;
+    g.bias_up = a->b_up_dev, g.g = p.g, g.u = p.u, g.h = p.h, g.h_ld = hidden_ld(a);
+    rc = gemm_pick<T, false, false, TOK_EPI_GLU>(g, "gated_ffn gate / up launch", stream);
+    if (rc != SR355_OK) return rc;
+    TokGemmArgs d = {};
+    d.n_jobs = 1, d.sections = 1, d.K = a->hidden;
+    TokJob &k = d.job[0];
+    k.a[0] = (const unsigned char *)p.h, k.a_ld = hidden_ld(a) * sizeof(T);
+    k.b[0] = (const unsigned char *)p.wd.p, k.b_ld = p.wd.ld * sizeof(T);
+    k.M = (int)a->rows, k.N = a->channels, k.bias = a->b_down_dev, k.c = a->y_dev, k.c_ld = a->channels;
+    return gemm_pick<T, false, false, TOK_EPI_STORE>(d, "gated_ffn down launch", stream);
+}
+
+template <typename T>
+int ffn_wgrad(const sr355_ffn_args *a, const BackwardPlan &p, hipStream_t stream) {
+    TokGemmArgs g = {};
+    g.sections = 1, g.K = (int)a->rows, g.splits = p.wgrad.splits, g.split_stages = p.wgrad.split_stages;
+    ReduceArgs r = {};
+    float *parts = p.parts;
+    const size_t n = (size_t)a->hidden * a->channels;
+    auto add = [&](const void *l, long long l_ld, const void *q, long long q_ld, int M, int N, void *out) {
+        if (!out) return;
+        TokJob &j = g.job[g.n_jobs];
+        j.a[0] = (const unsigned char *)l, j.a_ld = l_ld * sizeof(T);
+        j.b[0] = (const unsigned char *)q, j.b_ld = q_ld * sizeof(T);
+        j.M = M, j.N = N, j.c = out, j.c_ld = N, j.part = parts;
+        r.part[g.n_jobs] = parts, r.out[g.n_jobs] = out, r.n[g.n_jobs] = (long long)n;
+        if (parts) parts += p.wgrad.splits * n;
+        ++g.n_jobs;
+    };
+    add(p.dg, hidden_ld(a), p.x.p, p.x.ld, a->hidden, a->channels, a->dw_gate_dev);
+    add(p.du, hidden_ld(a), p.x.p, p.x.ld, a->hidden, a->channels, a->dw_up_dev);
+    add(p.dy.p, p.dy.ld, p.h, hidden_ld(a), a->channels, a->hidden, a->dw_down_dev);
+    if (!g.n_jobs) return SR355_OK;
+    const char *what = "gated_ffn weight gradient launch";
+    int rc;
+    if (p.wgrad.big) {
+        set_tiles<Tile256>(g, false);
+        rc = p.parts ? gemm_launch<T, Tile256, true, true, TOK_EPI_PART>(g, what, stream)
+                     : gemm_launch<T, Tile256, true, true, TOK_EPI_STORE>(g, what, stream);
+    } else {
+        set_tiles<Tile128>(g, false);
+        rc = p.parts ? gemm_launch<T, Tile128, true, true, TOK_EPI_PART>(g, what, stream)
+                     : gemm_launch<T, Tile128, true, true, TOK_EPI_STORE>(g, what, stream);
+    }
+    if (rc != SR355_OK || !p.parts) return rc;
+    r.splits = p.wgrad.splits;
+    const long long wgs = tok_cdiv((long long)n, 1024);
+    hipLaunchKernelGGL((reduce_splits_kernel<T>), dim3((unsigned)(wgs > 2048 ? 2048 : wgs), g.n_jobs), dim3(256), 0, stream, r);
+    return check_hip(hipGetLastError(), "gated_ffn weight gradient reduction launch");
+}
+
+template <typename T>
+int ffn_backward(const sr355_ffn_args *a, hipStream_t stream) {
+    BackwardPlan p(a, (unsigned char *)a->workspace_dev);
+    int rc = run_pads<T>(p, stream);
+    if (rc != SR355_OK) return rc;
+    if (p.need_hidden && a->rows > 0) {
+        TokGemmArgs g = {};
+        g.n_jobs = 1, g.sections = 1, g.act = a->activation, g.K = a->channels;
+        TokJob &j = g.job[0];
+        j.a[0] = (const unsigned char *)p.dy.p, j.a_ld = p.dy.ld * sizeof(T);
+        j.b[0] = (const unsigned char *)p.wd.p, j.b_ld = p.wd.ld * sizeof(T);
+        j.M = (int)a->rows, j.N = a->hidden;
+        g.g = p.dg, g.u = p.du, g.sg = p.g, g.su = p.u, g.h_ld = hidden_ld(a);
+        rc = gemm_pick<T, false, true, TOK_EPI_GLU_GRAD>(g, "gated_ffn hidden gradient launch", stream);
+        if (rc != SR355_OK) return rc;
+    }
+    if (a->dx_dev && a->rows > 0) {
+        TokGemmArgs g = {};
+        g.n_jobs = 1, g.sections = 2, g.K = a->hidden;
+        TokJob &j = g.job[0];
+        j.a[0] = (const unsigned char *)p.dg, j.a[1] = (const unsigned char *)p.du, j.a_ld = hidden_ld(a) * sizeof(T);
+        j.b[0] = (const unsigned char *)p.wg.p, j.b[1] = (const unsigned char *)p.wu.p, j.b_ld = p.wg.ld * sizeof(T);
+        j.M = (int)a->rows, j.N = a->channels, j.c = a->dx_dev, j.c_ld = a->channels;
+        rc = gemm_pick<T, false, true, TOK_EPI_STORE>(g, "gated_ffn data gradient launch", stream);
+        if (rc != SR355_OK) return rc;
+    }
+    rc = ffn_wgrad<T>(a, p, stream);
+    if (rc != SR355_OK || !p.col_parts) return rc;
+    constexpr int E = 16 / sizeof(T);
+    ColArgs c = {};
+    c.parts = p.col_parts, c.rows = a->rows, c.stride = 2 * hidden_ld(a) + p.dy.ld;
+    int n = 0, most = 0;
+    auto add = [&](const void *src, long long ld, long long first, int cols, const void *wanted) {
+        if (!wanted) return;
+        c.job[n++] = {src, ld, first, cols};
+        if (cols > most) most = cols;
+    };
+    add(p.dg, hidden_ld(a), 0, a->hidden, a->db_gate_dev);
+    add(p.du, hidden_ld(a), hidden_ld(a), a->hidden, a->db_up_dev);
+    add(p.dy.p, p.dy.ld, 2 * hidden_ld(a), a->channels, a->db_down_dev);
+    const int n_parts = (int)(tok_cdiv(a->rows, 8) < COL_PARTS ? tok_cdiv(a->rows, 8) : COL_PARTS);
+    if (n_parts > 0) {
+        hipLaunchKernelGGL((column_sums_kernel<T>), dim3(n_parts, (unsigned)tok_cdiv(most, 32 * E), n), dim3(256), 0, stream, c);
+        rc = check_hip(hipGetLastError(), "gated_ffn bias gradient launch");
+        if (rc != SR355_OK) return rc;
+    }
+    const long long first[3] = {0, hidden_ld(a), 2 * hidden_ld(a)};
+    const int count[3] = {a->hidden, a->hidden, a->channels};
+    void *const out[3] = {a->db_gate_dev, a->db_up_dev, a->db_down_dev};
+    return launch_tok_sum_parts(p.col_parts, n_parts, c.stride, first, count, out, 3, a->dtype, stream);
+}
+}  // namespace
+
+}  // namespace sr355
+
+using namespace sr355;
+
+extern "C" {
+
+size_t sr355_gated_ffn_saved_bytes(const sr355_ffn_args *a) {
+    if (!ffn_args_ok("gated_ffn_saved_bytes", a, false)) return 0;
+    return 3 * hidden_bytes(a) + 256;
+}
+
+size_t sr355_gated_ffn_workspace_bytes(const sr355_ffn_args *a, int backward) {
+    if (!ffn_args_ok("gated_ffn_workspace_bytes", a, backward != 0)) return 0;
+    return (backward ? BackwardPlan(a, nullptr).at : ForwardPlan(a, nullptr).at) + 256;
+}
+
+int sr355_gated_ffn_fwd(const sr355_ffn_args *a, void *stream) {
+    if (!ffn_args_ok("gated_ffn_fwd", a, false)) return SR355_ERR_INVALID;
+    if (a->rows == 0) return SR355_OK;
+    const size_t need = sr355_gated_ffn_workspace_bytes(a, 0);
+    if (!a->x_dev || !a->w_gate_dev || !a->w_up_dev || !a->w_down_dev || !a->y_dev || !a->workspace_dev ||
+        !tok_aligned16(a->workspace_dev) || a->workspace_bytes < need || !tok_aligned16(a->saved_dev) ||
+        (a->saved_dev && a->saved_bytes < sr355_gated_ffn_saved_bytes(a))) {
+        set_error("gated_ffn_fwd: null tensor, or workspace / saved buffer not 16-byte aligned or smaller than %zu / %zu bytes", need,
+                  sr355_gated_ffn_saved_bytes(a));
+        return SR355_ERR_INVALID;
+    }
+    if (a->dtype == SR355_DTYPE_F32) return ffn_forward<float>(a, (hipStream_t)stream);
+    if (a->dtype == SR355_DTYPE_BF16) return ffn_forward<bf16_t>(a, (hipStream_t)stream);
+    return ffn_forward<f16_t>(a, (hipStream_t)stream);
+}
+
+int sr355_gated_ffn_bwd(const sr355_ffn_args *a, void *stream) {
+    if (!ffn_args_ok("gated_ffn_bwd", a, true)) return SR355_ERR_INVALID;
+    const size_t need = sr355_gated_ffn_workspace_bytes(a, 1);
+    if ((a->rows > 0 && (!a->x_dev || !a->dy_dev || !a->saved_dev || a->saved_bytes < sr355_gated_ffn_saved_bytes(a))) ||
+        !tok_aligned16(a->saved_dev) || !a->w_gate_dev || !a->w_up_dev || !a->w_down_dev || !a->workspace_dev ||
+        !tok_aligned16(a->workspace_dev) || a->workspace_bytes < need) {
+        set_error("gated_ffn_bwd: null tensor, or workspace / saved buffer not 16-byte aligned or smaller than %zu / %zu bytes", need,
+                  sr355_gated_ffn_saved_bytes(a));
+        return SR355_ERR_INVALID;
+    }
+    if (a->dtype == SR355_DTYPE_F32) return ffn_backward<float>(a, (hipStream_t)stream);
+    if (a->dtype == SR355_DTYPE_BF16) return ffn_backward<bf16_t>(a, (hipStream_t)stream);
+    return ffn_backward<f16_t>(a, (hipStream_t)stream);
+}
+
+}  // extern "C"

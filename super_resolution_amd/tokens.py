@@ -1,0 +1,172 @@
+"""Operators on rows of channels ("tokens"): tensors ``[..., C]``, where the rows are an image's pixels or a sequence.
+
+``layer_norm``, ``gated_ffn`` and ``dropout`` are HIP kernels, forward and backward, in bfloat16, float16 and float32, with
+fp32 sums of a fixed order; ``FeedForwardBlock`` composes them into the channel-mixing half of a residual block,
+``x + dropout(gated_ffn(layer_norm(x)))``.  They stand beside the conv core's 3x3 convs, BatchNorm and residual adds:
+``rows_from_blocked`` and ``blocked_from_rows`` go between its blocked activations and rows.
+
+Any sizes, leading dimensions and strides are taken; what is not laid out as rows of contiguous channels is copied first.
+Widths that are multiples of 16 bytes are the fast ones.  All calls run on the current stream of their tensors' device, can
+be captured into a graph, and keep nothing between calls."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch import Tensor, nn
+from torch.autograd.function import once_differentiable
+
+from . import token_ops as ops
+
+
+def _recorded(*ts: Optional[Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: float) -> Tensor:
+        y, stats = ops.layer_norm_fwd_now(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, stats)
+        ctx.param_dtype = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy: Tensor):
+        x, weight, stats = ctx.saved_tensors
+        need = list(ctx.needs_input_grad[:3])
+        grads = ops.layer_norm_bwd_now(dy, x, weight, stats, ctx.param_dtype, need)
+        return (*(g if n else None for g, n in zip(grads, need)), None)
+
+
+def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5) -> Tensor:
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension of ``x``.  ``weight`` and ``bias``, ``[C]``,
+    are of x's type or float32 (both of one type), and so are their gradients.  A row of one channel or of equal channels
+    gives ``bias``."""
+    if _recorded(x, weight, bias):
+        return _LayerNorm.apply(x, weight, bias, eps)
+    return ops.layer_norm_fwd_now(x, weight, bias, eps, False)[0]
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x: Tensor, p: float, rng: Tensor, site: int, residual: Optional[Tensor]) -> Tensor:
+        ctx.save_for_backward(rng)
+        ctx.p, ctx.site = p, site
+        return ops.dropout_now(x, residual, p, rng, site)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy: Tensor):
+        (rng,) = ctx.saved_tensors
+        dx = ops.dropout_now(dy, None, ctx.p, rng, ctx.site) if ctx.needs_input_grad[0] else None
+        return dx, None, None, None, dy if ctx.needs_input_grad[4] else None
+
+
+def dropout(x: Tensor, p: float, rng: Tensor, site: int = 0, residual: Optional[Tensor] = None) -> Tensor:
+    """``x`` with each element dropped with probability ``p`` and the others divided by ``1 - p``, plus ``residual`` (x's
+    shape and type) where one is given.  No mask is stored: which elements stay is a function of the element's index in
+    ``x`` (row-major), the generator's state ``rng`` and ``site``, and the backward pass computes it again.
+
+    ``rng`` is an int64 tensor of two words on x's device, a seed and a step (modulo 2^32).  Calls that share both take
+    different ``site`` numbers or drop the same elements; a training loop advances the step.  The kernel reads ``rng`` when
+    it runs, so a captured graph's replays drop what the words say then; changing them in place between a call and its
+    backward pass is an error that autograd reports.  ``p`` counts in steps of 2^-16 and the scale is that of the nearest
+    step; a dropped infinity or NaN is dropped."""
+    if _recorded(x, residual):
+        return _Dropout.apply(x, p, rng, site, residual)
+    return ops.dropout_now(x, residual, p, rng, site)
+
+
+class _GatedFfn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, b_gate: Optional[Tensor],
+                b_up: Optional[Tensor], b_down: Optional[Tensor], activation: int) -> Tensor:
+        y, saved = ops.gated_ffn_fwd_now(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation, True)
+        ctx.save_for_backward(x, w_gate, w_up, w_down, saved)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy: Tensor):
+        need = list(ctx.needs_input_grad[:7])
+        grads = ops.gated_ffn_bwd_now(dy, *ctx.saved_tensors, ctx.activation, need)
+        return (*(g if n else None for g, n in zip(grads, need)), None)
+
+
+def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, b_gate: Optional[Tensor] = None,
+              b_up: Optional[Tensor] = None, b_down: Optional[Tensor] = None, activation: str = "silu") -> Tensor:
+    """``(act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down`` for rows ``x`` ``[..., C]``, ``w_gate`` and
+    ``w_up`` ``[F, C]`` and ``w_down`` ``[C, F]`` (``nn.Linear`` weights), all of x's type.  ``activation``: "silu", "gelu"
+    (by the error function), "relu" or "sigmoid".  Products accumulate in fp32; the hidden channels are held in x's type
+    between the launches.  A call that autograd records keeps three rows of F hidden channels per row of x."""
+    if activation not in ops.ACTIVATIONS:
+        raise RuntimeError(f"gated_ffn: activation must be one of {', '.join(ops.ACTIVATIONS)}, got {activation!r}")
+    code = ops.ACTIVATIONS[activation]
+    if _recorded(x, w_gate, w_up, w_down, b_gate, b_up, b_down):
+        return _GatedFfn.apply(x, w_gate, w_up, w_down, b_gate, b_up, b_down, code)
+    return ops.gated_ffn_fwd_now(x, w_gate, w_up, w_down, b_gate, b_up, b_down, code, False)[0]
+
+
+def rows_from_blocked(x: Tensor, channels: int) -> Tensor:
+    """The conv core's blocked activations ``[N, H, units, W, c]`` as rows ``[N, H, W, channels]`` (a copy)."""
+    if x.dim() != 5 or not 0 < channels <= x.shape[2] * x.shape[4]:
+        raise RuntimeError(f"rows_from_blocked: expected blocked activations of at least {channels} channels, got {tuple(x.shape)}")
+    N, H, U, W, c = x.shape
+    return x.permute(0, 1, 3, 2, 4).reshape(N, H, W, U * c)[..., :channels]
+
+
+def blocked_from_rows(x: Tensor) -> Tensor:
+    """bfloat16 rows ``[N, H, W, C]`` as the conv core's blocked activations ``[N, H, units, W, 8]``, zeros behind C."""
+    if x.dim() != 4 or x.dtype != torch.bfloat16:
+        raise RuntimeError(f"blocked_from_rows: expected bfloat16 rows [N, H, W, C], got {tuple(x.shape)} of {x.dtype}")
+    from .conv_core import units_for
+    N, H, W, c = x.shape
+    units = units_for(c)
+    if units * 8 != c:
+        x = nn.functional.pad(x, (0, units * 8 - c))
+    return x.reshape(N, H, W, units, 8).permute(0, 1, 3, 2, 4).contiguous()
+
+
+class FeedForwardBlock(nn.Module):
+    """``x + dropout(gated_ffn(layer_norm(x)))`` on rows ``[..., channels]``: the channel-mixing half of a residual block.
+
+    Parameters are float32; where x is bfloat16 or float16 the projections' are rounded to its type for the call (their
+    gradients come back as float32) and the normalisation's are used as they are.  In training mode with ``dropout > 0``
+    every call takes the seed and step of ``rng_state`` (a buffer that checkpoints carry; ``seed()`` sets it) and advances
+    the step, on the device, so that replays of a captured graph do too."""
+
+    def __init__(self, channels: int, hidden: int, dropout: float = 0.0, activation: str = "silu", bias: bool = True,
+                 eps: float = 1e-5):
+        super().__init__()
+        if channels < 1 or hidden < 1 or not 0.0 <= dropout <= 1.0 or activation not in ops.ACTIVATIONS:
+            raise ValueError(f"FeedForwardBlock: channels={channels}, hidden={hidden}, dropout={dropout}, activation={activation!r}")
+        self.channels, self.hidden, self.dropout, self.activation = channels, hidden, dropout, activation
+        self.norm = nn.LayerNorm(channels, eps=eps)
+        self.gate = nn.Linear(channels, hidden, bias=bias)
+        self.up = nn.Linear(channels, hidden, bias=bias)
+        self.down = nn.Linear(hidden, channels, bias=bias)
+        self.register_buffer("rng_state", torch.zeros(2, dtype=torch.int64))
+
+    def seed(self, seed: int) -> None:
+        """Start the dropout's generator at step 0 of ``seed``."""
+        with torch.no_grad():
+            self.rng_state.copy_(torch.tensor([seed, 0], dtype=torch.int64))
+
+    def forward(self, x: Tensor) -> Tensor:
+        if x.dim() < 1 or x.shape[-1] != self.channels:
+            raise RuntimeError(f"FeedForwardBlock: expected rows of {self.channels} channels, got {tuple(x.shape)}")
+
+        def typed(t: Optional[Tensor]) -> Optional[Tensor]:
+            return None if t is None else t.to(x.dtype)
+
+        h = layer_norm(x, self.norm.weight, self.norm.bias, self.norm.eps)
+        h = gated_ffn(h, typed(self.gate.weight), typed(self.up.weight), typed(self.down.weight), typed(self.gate.bias),
+                      typed(self.up.bias), typed(self.down.bias), self.activation)
+        if not self.training or self.dropout == 0.0:
+            return x + h
+        rng = self.rng_state.clone()          # what this call's backward pass reads, while the buffer moves on
+        self.rng_state[1].add_(1)
+        return dropout(h, self.dropout, rng, residual=x)

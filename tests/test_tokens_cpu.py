@@ -1,0 +1,123 @@
+"""CPU: the operators on rows of channels — fakes, argument checks of the Python and the C side, size queries.  No kernel
+runs here."""
+import ctypes as C
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from super_resolution_amd import _lib, token_ops, tokens
+from super_resolution_amd._lib import FfnArgs
+
+OPS = ("layer_norm_fwd", "layer_norm_bwd", "dropout", "gated_ffn_fwd", "gated_ffn_bwd")
+
+
+@pytest.fixture(scope="module")
+def L():
+    return _lib.lib()
+
+
+def test_every_op_is_registered_with_a_fake():
+    for name in OPS:
+        assert getattr(torch.ops.sr355, name).default._schema.name == f"sr355::{name}"
+        assert getattr(token_ops, name)._abstract_fn is not None
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_fakes_predict_shapes_and_types(dtype):
+    with FakeTensorMode():
+        x = torch.empty(3, 5, 24, dtype=dtype, device="cuda")
+        w32 = torch.empty(24, device="cuda")
+        y, stats = torch.ops.sr355.layer_norm_fwd(x, w32, w32, 1e-5, True)
+        assert y.shape == x.shape and y.dtype == dtype and stats.shape == (2, 15) and stats.dtype == torch.float32
+        dx, dw, db = torch.ops.sr355.layer_norm_bwd(y, x, w32, stats, torch.float32, [True, True, False])
+        assert dx.shape == x.shape and dw.shape == (24,) and dw.dtype == torch.float32 and db.shape == (0,)
+        rng = torch.empty(2, dtype=torch.int64, device="cuda")
+        assert torch.ops.sr355.dropout(x, None, 0.5, rng, 0).shape == x.shape
+        wg, wd = torch.empty(40, 24, dtype=dtype, device="cuda"), torch.empty(24, 40, dtype=dtype, device="cuda")
+        y, saved = torch.ops.sr355.gated_ffn_fwd(x, wg, wg, wd, None, None, None, 0, True)
+        assert y.shape == x.shape and saved.dtype == torch.uint8
+        assert saved.numel() >= 3 * 15 * 40 * x.element_size()
+        g = torch.ops.sr355.gated_ffn_bwd(y, x, wg, wg, wd, saved, 0, [True] * 7)
+        assert [tuple(t.shape) for t in g] == [(3, 5, 24), (40, 24), (40, 24), (24, 40), (40,), (40,), (24,)]
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(4, 8)
+    w = torch.zeros(8, 8)
+    for call in (lambda: tokens.layer_norm(x), lambda: tokens.gated_ffn(x, w, w, w),
+                 lambda: tokens.dropout(x, 0.5, torch.zeros(2, dtype=torch.int64)),
+                 lambda: tokens.FeedForwardBlock(8, 16)(x)):
+        with pytest.raises(RuntimeError, match="ROCm devices only"):
+            call()
+    with pytest.raises(RuntimeError, match="activation"):
+        tokens.gated_ffn(x, w, w, w, activation="tanh")
+    for bad in ({"channels": 0, "hidden": 4}, {"channels": 4, "hidden": 0}, {"channels": 4, "hidden": 4, "dropout": 1.5},
+                {"channels": 4, "hidden": 4, "activation": "tanh"}):
+        with pytest.raises(ValueError):
+            tokens.FeedForwardBlock(**bad)
+    with pytest.raises(RuntimeError, match="rows of 8"):
+        tokens.FeedForwardBlock(8, 16)(torch.zeros(4, 9))
+
+
+def test_block_layout_round_trip():
+    x = torch.randn(2, 3, 5, 24).to(torch.bfloat16)
+    b = tokens.blocked_from_rows(x)
+    assert b.shape == (2, 3, 4, 5, 8) and (b[:, :, 3] == 0).all()
+    assert torch.equal(tokens.rows_from_blocked(b, 24), x)
+    with pytest.raises(RuntimeError):
+        tokens.rows_from_blocked(b, 33)
+    with pytest.raises(RuntimeError):
+        tokens.blocked_from_rows(x.float())
+
+
+def test_c_entries_refuse_bad_arguments_without_touching_a_device(L):
+    p = 4096   # an address that nothing reads: every call below is refused before a launch
+    F = _lib.DTYPE_F32
+    assert L.sr355_layer_norm_fwd(None, 1, 8, 8, F, None, None, F, 1e-5, None, None, None, None) == -1
+    assert L.sr355_layer_norm_fwd(p, 1, 0, 8, F, None, None, F, 1e-5, p, None, None, None) == -1
+    assert L.sr355_layer_norm_fwd(p, 1, 8, 7, F, None, None, F, 1e-5, p, None, None, None) == -1        # stride < C
+    assert L.sr355_layer_norm_fwd(p, 1, 8, 8, 9, None, None, F, 1e-5, p, None, None, None) == -1        # type
+    assert L.sr355_layer_norm_fwd(p, -1, 8, 8, F, None, None, F, 1e-5, p, None, None, None) == -1
+    assert L.sr355_layer_norm_fwd(p, 1, 8, 8, F, p, None, _lib.DTYPE_BF16, 1e-5, p, None, None, None) == -1
+    assert L.sr355_layer_norm_fwd(p, 1, 8, 8, F, None, None, F, -1.0, p, None, None, None) == -1
+    assert L.sr355_layer_norm_fwd(p, 1, 8, 8, F, None, None, F, 1e-5, p, p, None, None) == -1           # mean without rstd
+    assert b"layer_norm_fwd" in L.sr355_last_error()
+    assert L.sr355_layer_norm_fwd(None, 0, 8, 8, F, None, None, F, 1e-5, None, None, None, None) == 0   # no rows: nothing to do
+    assert L.sr355_layer_norm_bwd_workspace_bytes(0) == 0 and L.sr355_layer_norm_bwd_workspace_bytes(8) > 0
+    assert L.sr355_layer_norm_bwd(p, 8, p, 8, 1, 8, F, None, F, p, p, p, p, p, None, 0, None) == -1     # no workspace
+    assert L.sr355_layer_norm_bwd(None, 8, p, 8, 1, 8, F, None, F, p, p, p, None, None, None, 0, None) == -1
+    assert L.sr355_layer_norm_bwd(None, 8, None, 8, 0, 8, F, None, F, None, None, None, None, None, None, 0, None) == 0
+    assert L.sr355_dropout(p, None, 8, F, 1.5, p, 0, p, None) == -1
+    assert L.sr355_dropout(p, None, 8, F, float("nan"), p, 0, p, None) == -1
+    assert L.sr355_dropout(p, None, 8, F, 0.5, None, 0, p, None) == -1
+    assert L.sr355_dropout(p, None, -1, F, 0.5, p, 0, p, None) == -1
+    assert L.sr355_dropout(None, None, 0, F, 0.5, None, 0, None, None) == 0
+
+    def ffn(**kw):
+        a = FfnArgs()
+        a.dtype, a.rows, a.channels, a.hidden, a.x_ld, a.dy_ld = F, 4, 8, 16, 8, 8
+        a.x_dev = a.w_gate_dev = a.w_up_dev = a.w_down_dev = a.y_dev = a.dy_dev = a.workspace_dev = a.saved_dev = p
+        a.workspace_bytes = a.saved_bytes = 1 << 30
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return C.byref(a)
+
+    assert L.sr355_gated_ffn_fwd(None, None) == -1 and L.sr355_gated_ffn_bwd(None, None) == -1
+    for kw in ({"dtype": 5}, {"activation": 4}, {"activation": -1}, {"rows": -1}, {"rows": 1 << 31}, {"channels": 0},
+               {"hidden": 0}, {"hidden": (1 << 20) + 1}, {"x_ld": 7}, {"x_dev": None}, {"w_gate_dev": None}, {"w_up_dev": None},
+               {"w_down_dev": None}, {"workspace_dev": None}, {"workspace_bytes": 16}, {"workspace_dev": p + 8},
+               {"saved_bytes": 16}, {"saved_dev": p + 4}):
+        assert L.sr355_gated_ffn_fwd(ffn(**kw), None) == -1, kw
+        assert L.sr355_gated_ffn_bwd(ffn(**kw), None) == -1, kw
+    assert L.sr355_gated_ffn_fwd(ffn(y_dev=None), None) == -1
+    assert L.sr355_gated_ffn_bwd(ffn(dy_dev=None), None) == -1
+    assert L.sr355_gated_ffn_bwd(ffn(saved_dev=None), None) == -1
+    assert L.sr355_gated_ffn_bwd(ffn(dy_ld=7), None) == -1
+    assert L.sr355_gated_ffn_fwd(ffn(rows=0), None) == 0
+    # what has to be padded (odd widths, an unaligned pointer) needs more room than what is read in place
+    base = L.sr355_gated_ffn_workspace_bytes(ffn(), 0)
+    assert L.sr355_gated_ffn_workspace_bytes(ffn(x_dev=p + 4), 0) > base
+    assert L.sr355_gated_ffn_workspace_bytes(ffn(x_ld=9), 0) > base
+    assert L.sr355_gated_ffn_workspace_bytes(ffn(rows=-1), 0) == 0
+    assert L.sr355_gated_ffn_saved_bytes(ffn()) >= 3 * 4 * 16 * 4
