@@ -4,10 +4,12 @@
 //     dWg = dg' x, dWu = du' x, dWd = dy' h, biases: column sums of dg, du, dy.
 // Forward: one launch computes both projections, the activation and the product (a workgroup multiplies its rows of x with
 // the gate and the up weights of the same hidden channels, so g and u meet in a wave's registers), one the projection back.
-// Backward: one launch computes dh and, in its epilogue, dg and du; one dx over both sections of k; one all three weight
-// gradients.  Products accumulate in fp32.  Between the launches g, u, h, dg and du are held in the type of x: as products'
-// operands they are rounded to it in any case, and g and u kept in fp32 would double the traffic of the two launches that
-// are nearest to the memory's pace.  Training keeps g, u and h (three rows of hidden channels each); inference h alone.
+// Training keeps act(g), u act'(g) and h, inference h alone.  Backward: one launch computes dh and, in its epilogue, dg and
+// du (two products per element: the derivative is taken in the forward pass, from g and u as they were accumulated); one dx,
+// over both sections of k; one all three weight gradients.  Products accumulate in fp32.  Between the launches the hidden
+// channels are held in the type of x: h, dg and du are rounded to it as operands of products in any case, and the two kept
+// factors in fp32 would double the traffic of the two launches that are nearest to the memory's pace (134 MB per array for
+// 16384 rows of 4096).
 //
 // Operands are read 16 bytes at a time.  What does not allow that (a width, stride or pointer that is no multiple of 16
 // bytes) is first copied into padded rows of the workspace, one launch for all of them.
@@ -16,9 +18,16 @@
 namespace sr355 {
 
 namespace {
-// tiles: 256 x 256 with eight waves where that fills the chip, else 128 x 128 with four waves, two workgroups per CU
-typedef TokTile<256, 256, 2, 4, 2> Tile256;
-typedef TokTile<128, 128, 2, 2, 2> Tile128;
+// 256 x 256 tiles where they fill the chip, one workgroup per CU; else 128 x 128, two per CU.  A row's share of a stage is a
+// whole 128-byte line where k is contiguous (with 64 bytes every line comes twice from the L2: 147 against 138 us for
+// 16384 x 4096 times 4096 x 1024); where k is strided a stage's rows are lines in any case, and five stages of 64 bytes hide
+// more latency than two of 128 (443 against 472 us for the three weight gradients of 16384 x 1024 x 4096).
+typedef TokTile<256, 256, 2, 4, 128, 2> Tile256;
+typedef TokTile<256, 256, 2, 4, 64, 5> TileWgrad;
+#ifndef T128
+#define T128 128, 128, 2, 2, 128, 2
+#endif
+typedef TokTile<T128> Tile128;
 constexpr int N_CU = 256;
 
 struct PadJob {
@@ -65,11 +74,14 @@ __global__ __launch_bounds__(256) void reduce_splits_kernel(ReduceArgs a) {
         if (vec) {
             for (int s = 0; s < a.splits; ++s) {
                 float t[4];
-                tok_load4<float>(part + (size_t)s * n + i, t);
+                tok_load<float, 4>(part + (size_t)s * n + i, t);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[j] += t[j];
             }
-            tok_store4<T>(out + i, v);
+            T o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = (T)v[j];
+            __builtin_memcpy(__builtin_assume_aligned(out + i, 4 * sizeof(T)), o, 4 * sizeof(T));
         } else {
             for (int j = 0; j < 4 && i + j < n; ++j) {
                 for (int s = 0; s < a.splits; ++s) v[j] += part[(size_t)s * n + i + j];
@@ -201,7 +213,8 @@ int run_pads(const Plan &plan, hipStream_t stream) {
     return check_hip(hipGetLastError(), "gated_ffn row padding launch");
 }
 
-long long hidden_ld(const sr355_ffn_args *a) { return round_up(a->hidden, a->dtype == SR355_DTYPE_F32 ? 4 : 8); }
+// rows of g, u, h, dg, du: whole groups of eight channels, what a lane of the epilogue stores
+long long hidden_ld(const sr355_ffn_args *a) { return round_up(a->hidden, 8); }
 
 size_t hidden_bytes(const sr355_ffn_args *a) {
     return ((size_t)a->rows * hidden_ld(a) * tok_type_bytes(a->dtype) + 255) & ~(size_t)255;
@@ -239,10 +252,10 @@ long long wgrad_tiles(const sr355_ffn_args *a) {
     return (a->dw_gate_dev ? f_c : 0) + (a->dw_up_dev ? f_c : 0) + (a->dw_down_dev ? c_f : 0);
 }
 WgradShape wgrad_shape(const sr355_ffn_args *a) {
-    const long long stages = tok_cdiv(a->rows, 128 / (long long)tok_type_bytes(a->dtype));
     WgradShape w;
-    w.big = wgrad_tiles<Tile256>(a) >= N_CU / 4;
-    const long long tiles = w.big ? wgrad_tiles<Tile256>(a) : wgrad_tiles<Tile128>(a);
+    w.big = wgrad_tiles<TileWgrad>(a) >= N_CU / 4;
+    const long long stages = tok_cdiv(a->rows, (w.big ? TileWgrad::KB : Tile128::KB) / (long long)tok_type_bytes(a->dtype));
+    const long long tiles = w.big ? wgrad_tiles<TileWgrad>(a) : wgrad_tiles<Tile128>(a);
     const long long want = tok_cdiv(w.big ? N_CU : 2 * N_CU, tiles < 1 ? 1 : tiles);
     long long splits = stages / 8 < want ? stages / 8 : want;
     if (splits < 1) splits = 1;
@@ -345,9 +358,9 @@ int ffn_wgrad(const sr355_ffn_args *a, const BackwardPlan &p, hipStream_t stream
     const char *what = "gated_ffn weight gradient launch";
     int rc;
     if (p.wgrad.big) {
-        set_tiles<Tile256>(g, false);
-        rc = p.parts ? gemm_launch<T, Tile256, true, true, TOK_EPI_PART>(g, what, stream)
-                     : gemm_launch<T, Tile256, true, true, TOK_EPI_STORE>(g, what, stream);
+        set_tiles<TileWgrad>(g, false);
+        rc = p.parts ? gemm_launch<T, TileWgrad, true, true, TOK_EPI_PART>(g, what, stream)
+                     : gemm_launch<T, TileWgrad, true, true, TOK_EPI_STORE>(g, what, stream);
     } else {
         set_tiles<Tile128>(g, false);
         rc = p.parts ? gemm_launch<T, Tile128, true, true, TOK_EPI_PART>(g, what, stream)

@@ -2,17 +2,20 @@
 // operand stored with k contiguous ("KC": activations against weights) or with its rows contiguous ("RC": k strided, what
 // the data and weight gradients read).  bf16 / fp16 on 32x32x16, fp32 on 32x32x2, fp32 accumulation.
 //
-// A workgroup computes BM x BN; its waves form a WM x WN grid.  A stage is 128 bytes of k per row, copied from memory
-// straight into the LDS (16 bytes a lane, no registers), STAGES of them in a ring: while stage t is multiplied the next
-// ones are in flight behind a counted wait, one barrier per stage.  What lies outside a matrix is read with an offset
-// beyond the buffer's end, which returns zeros, so edges need no branches and every wave issues the same number of copies.
-// The LDS image is permuted so that reads spread over the banks: KC tiles (rows of 8 units of 16 bytes) hold unit u of row
-// r at u ^ (r & 7); RC tiles of 16-bit types hold each 32-byte granule at g ^ f(k), f even, and are read by the transposing
+// A workgroup computes BM x BN; its waves form a WM x WN grid.  A stage is 64 or 128 bytes of k per row, copied from memory
+// straight into the LDS (16 bytes a lane, no registers), STAGES of them in a ring: while stage t is multiplied the next ones
+// are in flight behind a counted wait, one barrier per stage.  What lies outside a matrix is read with an offset beyond the
+// buffer's end, which returns zeros, so edges need no branches and every wave issues the same number of copies.
+// The LDS image is permuted so that reads spread over the banks: KC tiles hold unit u (16 bytes) of row r at u ^ rot(r); RC
+// tiles of 16-bit types hold each 32-byte granule at g ^ swz(k), swz even, and are read by the transposing
 // ds_read_b64_tr_b16.  The copies' destination is fixed (lane order), so the permutation is applied to their sources.
-// LDS reads are inline asm: a read that the compiler sees is put behind ALL copies in flight.  The reads of one k step are
-// issued before the MFMAs of the step in front of it and waited for by count.
-// The operands of the MFMA are exchanged (B first): a lane then holds four consecutive n of one m, what a row-major store
-// wants.
+// LDS reads are inline asm: a read that the compiler sees is put behind ALL copies in flight.
+// The operands of the MFMA are exchanged (B first): a lane then holds four consecutive n of one m.
+// Measured (bf16, 16384 x 4096 times 4096 x 1024, 256 x 256 tiles of 8 waves): 111 us = 1,240 TFLOP/s with the input in the
+// last-level cache, 134 us behind the kernels that write it; the matrix pipes are busy 66 % of the cycles and the clock
+// falls to 1.7-1.9 GHz, so what is left is bound by power: copies two stages further ahead took 15 % fewer cycles and 5 %
+// less time.  Four waves of 128 x 128 (half the LDS reads) take the same time; two workgroups per CU on 128 x 256 (64-byte
+// stages, half a cache line per row) 25 % more.
 #pragma once
 #include "token_common.h"
 
@@ -44,22 +47,28 @@ struct TokGemmArgs {
     int splits, split_stages;           // stages of one split
     int act;
     const void *bias_up;                // GLU
-    void *g, *u, *h;                    // GLU: saved (may be null) and product; gradient: dg, du (in g, u)
-    const void *sg, *su;                // gradient: saved g and u
+    void *g, *u, *h;                    // GLU: act(g), u act'(g) (both or none) and the product; gradient: dg, du (in g, u)
+    const void *sg, *su;                // gradient: act(g), u act'(g)
     long long h_ld;                     // elements, of g / u / h / dg / du; a multiple of 16 bytes
 };
 
 enum { TOK_EPI_STORE = 0, TOK_EPI_PART = 1, TOK_EPI_GLU = 2, TOK_EPI_GLU_GRAD = 3 };
 
-template <int BM_, int BN_, int WM_, int WN_, int STAGES_>
+template <int BM_, int BN_, int WM_, int WN_, int KB_, int STAGES_>
 struct TokTile {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STAGES = STAGES_;
+    static constexpr int KB = KB_;                                  // bytes of k of a stage, 64 or 128
+    static constexpr int KS = KB / 32;                              // its k steps
     static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
     static constexpr int MT = BM / WM / 32, NT = BN / WN / 32;      // 32 x 32 fragments of a wave
-    static constexpr int COPIES_A = BM / 8, COPIES_B = BN / 8;      // 1024-byte copies of a stage
+    static constexpr int COPIES_A = BM * KB / 1024, COPIES_B = BN * KB / 1024;   // 1024-byte copies of a stage
     static constexpr int COPIES = (COPIES_A + COPIES_B) / WAVES;    // of one wave
-    static constexpr int STAGE_BYTES = (BM + BN) * 128;
+    static constexpr int STAGE_BYTES = (BM + BN) * KB;
+    static constexpr int TURN_ROW = NT * 32 * 4;                    // a row of a wave's fp32 results on their way out
+    static constexpr int TURN = STAGES * STAGE_BYTES / WAVES / (32 * TURN_ROW) < MT ? STAGES * STAGE_BYTES / WAVES / (32 * TURN_ROW) : MT;
     static constexpr int LDS_BYTES = STAGES * STAGE_BYTES;
+    static_assert(TURN > 0 && MT % TURN == 0, "the results turn in the stages' memory, TURN fragments at a time");
+    static_assert(KS % 2 == 0, "the fragments alternate");
     static_assert(COPIES_A % WAVES == 0 && COPIES_B % WAVES == 0, "a wave's k-th copy belongs to one operand");
     static_assert(LDS_BYTES <= 160 * 1024, "LDS");
 };
@@ -83,10 +92,11 @@ __device__ __forceinline__ void tok_mfma(const tok_v4u &b, const tok_v4u &a, tok
 }
 
 // Geometry of one operand's LDS image: R rows of the output side, T elements.
-template <typename T, int R, bool RC>
+template <typename T, int R, int KB, bool RC>
 struct TokImage {
     static constexpr int E = 16 / sizeof(T);
-    static constexpr int BK = 128 / sizeof(T);
+    static constexpr int BK = KB / sizeof(T);
+    static constexpr int ROW_UNITS = KB / 16;                        // KC: units of a row
     static constexpr int K_BYTES = R * sizeof(T);                    // RC: one k of the image
     static constexpr int UNITS = K_BYTES / 16;
     static constexpr int GRANULES = K_BYTES / 32;
@@ -95,11 +105,14 @@ struct TokImage {
     static __device__ __forceinline__ int swz(int k) {
         return sizeof(T) == 4 ? 0 : (GRANULES >= 8 ? 2 * (k & 3) : (GRANULES >= 4 ? 2 * ((k >> 1) & 1) : 0));
     }
+    // KC: permutation of the units of row r.  A 16-byte read goes through the 64 banks 16 lanes at a time (lanes 0-3, 12-15,
+    // 20-27 and 4-11, 16-19, 28-31 of a half wave): their 16 rows then lie at 16 different places of 256 bytes.
+    static __device__ __forceinline__ int rot(int r) { return ROW_UNITS == 8 ? (r >> 1) & 7 : (r >> 2) & 3; }
     // copy j of the image: the row (KC) or k (RC) that lane `lane` brings, and its unit
     static __device__ __forceinline__ void source(int j, int lane, int &line, int &unit) {
         if constexpr (!RC) {
-            line = 8 * j + (lane >> 3);
-            unit = (lane & 7) ^ (lane >> 3);
+            line = (j * 64 + lane) / ROW_UNITS;
+            unit = (lane % ROW_UNITS) ^ rot(line);
         } else {
             const int at = j * 64 + lane;                            // unit of the image
             line = at / UNITS;
@@ -136,63 +149,47 @@ __device__ __forceinline__ float tok_gauss(float g) {      // exp(-g^2 / 2)
     if constexpr (EXACT) return expf(-0.5f * g * g);
     return __builtin_amdgcn_exp2f(-0.72134752044448f * g * g);
 }
-template <bool EXACT>
-__device__ __forceinline__ float tok_act(int kind, float g) {
-    if (kind == SR355_ACT_SILU) return g * tok_sigmoid<EXACT>(g);
-    if (kind == SR355_ACT_GELU) return g * (0.5f * (1.0f + erff(0.70710678118655f * g)));
-    if (kind == SR355_ACT_RELU) return g < 0.f ? 0.f : g;             // (a NaN stays one)
+template <bool EXACT, int KIND>
+__device__ __forceinline__ float tok_act(float g) {
+    if constexpr (KIND == SR355_ACT_SILU) return g * tok_sigmoid<EXACT>(g);
+    if constexpr (KIND == SR355_ACT_GELU) return g * (0.5f * (1.0f + erff(0.70710678118655f * g)));
+    if constexpr (KIND == SR355_ACT_RELU) return g < 0.f ? 0.f : g;       // (a NaN stays one)
     return tok_sigmoid<EXACT>(g);
 }
-template <bool EXACT>
-__device__ __forceinline__ void tok_act_grad(int kind, float g, float &a, float &da) {
-    if (kind == SR355_ACT_SILU) {
+template <bool EXACT, int KIND>
+__device__ __forceinline__ void tok_act_grad(float g, float &a, float &da) {
+    if constexpr (KIND == SR355_ACT_SILU) {
         const float s = tok_sigmoid<EXACT>(g);
         a = g * s, da = s * (1.0f + g * (1.0f - s));
-    } else if (kind == SR355_ACT_GELU) {
+    } else if constexpr (KIND == SR355_ACT_GELU) {
         const float cdf = 0.5f * (1.0f + erff(0.70710678118655f * g));
         a = g * cdf, da = cdf + g * (0.39894228040143f * tok_gauss<EXACT>(g));
-    } else if (kind == SR355_ACT_RELU) {
+    } else if constexpr (KIND == SR355_ACT_RELU) {
         a = g < 0.f ? 0.f : g, da = g > 0.f ? 1.0f : 0.f;
     } else {
         a = tok_sigmoid<EXACT>(g), da = a * (1.0f - a);
     }
 }
 
-// Four consecutive elements.
+// Eight consecutive elements, in 16-byte accesses.
 template <typename T>
-__device__ __forceinline__ void tok_store4(T *p, const float (&v)[4]) {
-    T t[4];
+__device__ __forceinline__ void tok_store8(T *p, const float (&v)[8]) {
+    constexpr int E = 16 / sizeof(T);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) t[j] = (T)v[j];
-    if constexpr (sizeof(T) == 2) {
-        tok_v2u raw;
-        __builtin_memcpy(&raw, t, 8);
-        *reinterpret_cast<tok_v2u *>(p) = raw;
-    } else {
-        tok_v4u raw;
-        __builtin_memcpy(&raw, t, 16);
-        *reinterpret_cast<tok_v4u *>(p) = raw;
-    }
+    for (int j = 0; j < 8; j += E) tok_store<T, E>(p + j, *reinterpret_cast<const float(*)[E]>(v + j));
 }
 template <typename T>
-__device__ __forceinline__ void tok_load4(const T *p, float (&v)[4]) {
-    T t[4];
-    if constexpr (sizeof(T) == 2) {
-        const tok_v2u raw = *reinterpret_cast<const tok_v2u *>(p);
-        __builtin_memcpy(t, &raw, 8);
-    } else {
-        const tok_v4u raw = *reinterpret_cast<const tok_v4u *>(p);
-        __builtin_memcpy(t, &raw, 16);
-    }
+__device__ __forceinline__ void tok_load8(const T *p, float (&v)[8]) {
+    constexpr int E = 16 / sizeof(T);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = (float)t[j];
+    for (int j = 0; j < 8; j += E) tok_load<T, E>(p + j, *reinterpret_cast<float(*)[E]>(v + j));
 }
 
 template <typename T, typename G, bool A_RC, bool B_RC, int EPI>
 __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
-    typedef TokImage<T, G::BM, A_RC> IA;
-    typedef TokImage<T, G::BN, B_RC> IB;
-    constexpr int BK = IA::BK, E = IA::E, KS = 4;          // four k steps of 32 bytes per stage
+    typedef TokImage<T, G::BM, G::KB, A_RC> IA;
+    typedef TokImage<T, G::BN, G::KB, B_RC> IB;
+    constexpr int BK = IA::BK, E = IA::E, KS = G::KS;
     constexpr int MT = G::MT, NT = G::NT;
     constexpr unsigned OUT = 0x80000000u;                  // an offset beyond every buffer
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
@@ -247,8 +244,9 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
             vb[i] = n0 + unit * E < job.N ? (unsigned)(line * job.b_ld + unit * 16) : OUT;
             kb[i] = line;
         } else {
-            // GLU: blocks of 64 image rows = 32 gate rows, then 32 up rows (a copy's eight rows are of one kind)
-            const int row = EPI == TOK_EPI_GLU ? (line >> 6) * 32 + (line & 31) : line;
+            // GLU: a wave's NT * 32 image rows are NT * 16 gate rows, then the up rows of the same hidden channels (a copy's
+            // eight rows are of one kind)
+            const int row = EPI == TOK_EPI_GLU ? (line / (NT * 32)) * (NT * 16) + line % (NT * 16) : line;
             vb[i] = n0 + row < job.N ? (unsigned)(row * job.b_ld + unit * 16) : OUT;
             kb[i] = unit * E;
         }
@@ -261,44 +259,39 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
         t1 = t0 + p.split_stages < t1 ? t0 + p.split_stages : t1;
     }
 
-    auto copy_stage = [&](int t, int slot) {
-        const bool live = t < t1;
-        const int sec = t >= n_stage ? 1 : 0;
-        const int k0 = (t - sec * n_stage) * BK;
-        const unsigned char *pa = job.a[EPI == TOK_EPI_GLU ? 0 : sec], *pb = job.b[EPI == TOK_EPI_GLU ? 0 : sec];
-        const long long ao = A_RC ? k0 * job.a_ld + m0 * (long long)sizeof(T) : m0 * job.a_ld + k0 * (long long)sizeof(T);
-        const long long bo = B_RC ? k0 * job.b_ld + n0 * (long long)sizeof(T) : n0 * job.b_ld + k0 * (long long)sizeof(T);
-        const int size = live ? 0x7fffffff : 0;
-        __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char *>(pa + ao), 0, size, 0x00020000);
-        __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char *>(pb + bo), 0, size, 0x00020000);
-        __amdgpu_buffer_rsrc_t rb2 = rb;
-        if (EPI == TOK_EPI_GLU)
-            rb2 = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char *>(job.b[1] + bo), 0, size, 0x00020000);
-        unsigned char *dst = smem + slot * G::STAGE_BYTES + wave * 1024;
-        const int left = p.K - k0;
-        if (left >= BK) {
-#pragma unroll
-            for (int i = 0; i < CA; ++i)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (tok_lds_void *)(dst + i * G::WAVES * 1024), 16, va[i], 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < CB; ++i) {
-                const bool up = EPI == TOK_EPI_GLU && (((i * G::WAVES + wave) >> 2) & 1);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(up ? rb2 : rb, (tok_lds_void *)(dst + G::BM * 128 + i * G::WAVES * 1024), 16,
-                                                         vb[i], 0, 0, 0);
-            }
+    // The next stage to copy: its number, operands' corners, k that is left of its section.
+    const long long a_step = A_RC ? BK * job.a_ld : G::KB, b_step = B_RC ? BK * job.b_ld : G::KB;
+    const long long a_corner = A_RC ? m0 * (long long)sizeof(T) : m0 * job.a_ld;
+    const long long b_corner = B_RC ? n0 * (long long)sizeof(T) : n0 * job.b_ld;
+    const unsigned char *pa = job.a[0] + a_corner + t0 * a_step, *pb = job.b[0] + b_corner + t0 * b_step;
+    const long long up_off = job.b[1] - job.b[0];          // GLU: both weights' rows are of one stride
+    const unsigned char *const pa1 = job.a[1] + a_corner, *const pb1 = job.b[1] + b_corner;
+    const int sections = EPI == TOK_EPI_STORE ? p.sections : 1;
+    int copy_t = t0, left = p.K - t0 * BK;
+    const int K = p.K;
+    // Copy I of this wave's CA + CB copies of the stage.  Past the last stage it copies zeros, so that the counted waits always
+    // see the same number of copies.
+    auto copy_one = [&](int slot, auto which) {
+        constexpr int I = decltype(which)::value;
+        const int size = copy_t < t1 ? 0x7fffffff : 0;
+        unsigned char *const dst = smem + slot * G::STAGE_BYTES + wave * 1024;
+        if constexpr (I < CA) {
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char *>(pa), 0, size, 0x00020000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (tok_lds_void *)(dst + I * G::WAVES * 1024), 16, ka[I] < left ? va[I] : OUT, 0, 0, 0);
         } else {
-#pragma unroll
-            for (int i = 0; i < CA; ++i)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (tok_lds_void *)(dst + i * G::WAVES * 1024), 16,
-                                                         ka[i] < left ? va[i] : OUT, 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < CB; ++i) {
-                const bool up = EPI == TOK_EPI_GLU && (((i * G::WAVES + wave) >> 2) & 1);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(up ? rb2 : rb, (tok_lds_void *)(dst + G::BM * 128 + i * G::WAVES * 1024), 16,
-                                                         kb[i] < left ? vb[i] : OUT, 0, 0, 0);
-            }
+            constexpr int J = I - CA;
+            const unsigned char *q = pb;
+            if (EPI == TOK_EPI_GLU && (((J * G::WAVES + wave) * (1024 / G::KB) / (NT * 16)) & 1)) q += up_off;
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char *>(q), 0, size, 0x00020000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (tok_lds_void *)(dst + G::BM * G::KB + J * G::WAVES * 1024), 16,
+                                                     kb[J] < left ? vb[J] : OUT, 0, 0, 0);
+        }
+        if constexpr (I + 1 == CA + CB) {
+            ++copy_t, left -= BK, pa += a_step, pb += b_step;
+            if (sections == 2 && copy_t == n_stage) pa = pa1, pb = pb1, left = K;
         }
     };
+    auto copy_stage = [&](int slot) { tok_static_for<CA + CB>([&](auto i) { copy_one(slot, i); }); };
 
     // Addresses of this lane's reads inside a stage.
     const unsigned lds0 = (unsigned)(size_t)(tok_lds_void *)smem;
@@ -308,7 +301,7 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
         const int g4 = lane >> 4, q = (lane & 15) >> 2, pp = lane & 3;
         if constexpr (!A_RC) {
 #pragma unroll
-            for (int s = 0; s < KS; ++s) ra_off[s] = (wm * MT * 32 + c) * 128 + (((2 * s + half) ^ (c & 7)) * 16);
+            for (int s = 0; s < KS; ++s) ra_off[s] = (wm * MT * 32 + c) * G::KB + (((2 * s + half) ^ IA::rot(c)) * 16);
         } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
             for (int i = 0; i < MT; ++i)
@@ -319,14 +312,14 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
         }
         if constexpr (!B_RC) {
 #pragma unroll
-            for (int s = 0; s < KS; ++s) rb_off[s] = G::BM * 128 + (wn * NT * 32 + c) * 128 + (((2 * s + half) ^ (c & 7)) * 16);
+            for (int s = 0; s < KS; ++s) rb_off[s] = G::BM * G::KB + (wn * NT * 32 + c) * G::KB + (((2 * s + half) ^ IB::rot(c)) * 16);
         } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
             for (int i = 0; i < NT; ++i)
-                rb_off[i] = G::BM * 128 + (8 * (g4 >> 1) + q) * IB::K_BYTES + ((((wn * NT + i) * 2 + (g4 & 1)) ^ IB::swz(q)) * 32) + pp * 8;
+                rb_off[i] = G::BM * G::KB + (8 * (g4 >> 1) + q) * IB::K_BYTES + ((((wn * NT + i) * 2 + (g4 & 1)) ^ IB::swz(q)) * 32) + pp * 8;
         } else {
 #pragma unroll
-            for (int i = 0; i < NT; ++i) rb_off[i] = G::BM * 128 + 4 * half * IB::K_BYTES + ((wn * NT + i) * 32 + c) * 4;
+            for (int i = 0; i < NT; ++i) rb_off[i] = G::BM * G::KB + 4 * half * IB::K_BYTES + ((wn * NT + i) * 32 + c) * 4;
         }
     }
 
@@ -344,40 +337,34 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
         tok_v2u alo[MT], ahi[MT], blo[NT], bhi[NT];
         float a4[MT][4], b4[NT][4];
     } fr[2];
-    auto read_step = [&](Frags &f, unsigned base, auto step) {
+    // fragment X (A's, then B's) of k step S; a template, since the offsets are immediates of the instructions
+    auto read_one = [&](Frags &f, unsigned base, auto step, auto which) {
         constexpr int S = decltype(step)::value;
-        // (a template loop: the offsets are immediates of the instructions)
-        auto one = [&](auto which, auto index) {
-            constexpr bool IS_A = decltype(which)::value == 0;
-            constexpr int X = decltype(index)::value;
-            typedef typename std::conditional<IS_A, IA, IB>::type I;
-            constexpr bool RC = IS_A ? A_RC : B_RC;
-            const unsigned *off = IS_A ? ra_off : rb_off;
-            if constexpr (!RC) {
-                tok_read<T, I, false, X * 32 * 128>(IS_A ? f.a[IS_A ? X : 0] : f.b[IS_A ? 0 : X], f.alo[0], f.ahi[0], base + off[S]);
-            } else if constexpr (sizeof(T) == 2) {
-                tok_v4u dummy;
-                tok_read<T, I, true, S * 16 * I::K_BYTES>(dummy, IS_A ? f.alo[IS_A ? X : 0] : f.blo[IS_A ? 0 : X],
-                                                          IS_A ? f.ahi[IS_A ? X : 0] : f.bhi[IS_A ? 0 : X], base + off[X]);
-            } else {
-                float(&v)[4] = IS_A ? f.a4[IS_A ? X : 0] : f.b4[IS_A ? 0 : X];
-                asm volatile(
-                    "ds_read_b32 %0, %4 offset:%5\n\tds_read_b32 %1, %4 offset:%6\n\t"
-                    "ds_read_b32 %2, %4 offset:%7\n\tds_read_b32 %3, %4 offset:%8"
-                    : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
-                    : "v"(base + off[X]), "n"((8 * S + 0) * I::K_BYTES), "n"((8 * S + 1) * I::K_BYTES), "n"((8 * S + 2) * I::K_BYTES),
-                      "n"((8 * S + 3) * I::K_BYTES)
-                    : "memory");
-            }
-        };
-        tok_static_for<MT>([&](auto i) { one(std::integral_constant<int, 0>{}, i); });
-        tok_static_for<NT>([&](auto i) { one(std::integral_constant<int, 1>{}, i); });
+        constexpr bool IS_A = decltype(which)::value < MT;
+        constexpr int X = IS_A ? decltype(which)::value : decltype(which)::value - MT;
+        typedef typename std::conditional<IS_A, IA, IB>::type I;
+        constexpr bool RC = IS_A ? A_RC : B_RC;
+        const unsigned *off = IS_A ? ra_off : rb_off;
+        if constexpr (!RC) {
+            tok_read<T, I, false, X * 32 * G::KB>(IS_A ? f.a[IS_A ? X : 0] : f.b[IS_A ? 0 : X], f.alo[0], f.ahi[0], base + off[S]);
+        } else if constexpr (sizeof(T) == 2) {
+            tok_v4u dummy;
+            tok_read<T, I, true, S * 16 * I::K_BYTES>(dummy, IS_A ? f.alo[IS_A ? X : 0] : f.blo[IS_A ? 0 : X],
+                                                      IS_A ? f.ahi[IS_A ? X : 0] : f.bhi[IS_A ? 0 : X], base + off[X]);
+        } else {
+            float(&v)[4] = IS_A ? f.a4[IS_A ? X : 0] : f.b4[IS_A ? 0 : X];
+            asm volatile(
+                "ds_read_b32 %0, %4 offset:%5\n\tds_read_b32 %1, %4 offset:%6\n\t"
+                "ds_read_b32 %2, %4 offset:%7\n\tds_read_b32 %3, %4 offset:%8"
+                : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])
+                : "v"(base + off[X]), "n"((8 * S + 0) * I::K_BYTES), "n"((8 * S + 1) * I::K_BYTES), "n"((8 * S + 2) * I::K_BYTES),
+                  "n"((8 * S + 3) * I::K_BYTES)
+                : "memory");
+        }
     };
-    // at most PENDING younger LDS instructions outstanding, then the fragments may be used
-    constexpr int STEP_READS = MT * IA::READS + NT * IB::READS;
-    auto settle = [&](Frags &f, auto pending) {
-        constexpr int P = decltype(pending)::value < 15 ? decltype(pending)::value : 15;
-        asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(P) : "memory");
+    // all LDS reads have returned: the fragments may be used
+    auto settle = [&](Frags &f) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             if constexpr (!A_RC) {
@@ -403,124 +390,184 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
             }
         }
     };
-    auto multiply = [&](const Frags &f) {
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) tok_mfma<T>(f.b[j], f.a[i], acc[i][j]);
-    };
 
-    constexpr int AHEAD = G::STAGES - 1;
+    // One wave's MFMAs of a k step leave the matrix pipe idle for every other instruction that stands between two steps, so
+    // everything else stands between the MFMAs, and sched_barrier keeps it there: behind the first ones the reads of the next
+    // step, behind the others copies.  In front of the first read of stage t + 1, which is in the last step of stage t,
+    // stage t + 1 has to be there and every wave to be done reading stage t: a counted wait and the barrier, one per stage.
+    // From there on the slot of stage t takes stage t + STAGES: a first part of the copies in that step, the rest in the
+    // first step of stage t + 1.
+    constexpr int MFMAS = MT * NT, READS = MT + NT;
+    constexpr int FIRST_PART = (CA + CB) / 2;
+    constexpr int READ_SLOTS = READS < MFMAS ? READS : MFMAS, COPY_SLOT = READ_SLOTS < MFMAS ? READ_SLOTS : 0;
 #pragma unroll
-    for (int s = 0; s < AHEAD; ++s) copy_stage(t0 + s, s);
+    for (int s = 0; s + 1 < G::STAGES; ++s) copy_stage(s);
+    tok_static_for<FIRST_PART>([&](auto i) { copy_one(G::STAGES - 1, i); });
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((G::STAGES - 2) * (CA + CB) + FIRST_PART) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
     int slot = 0;
+    if (t0 < t1) tok_static_for<READS>([&](auto x) { read_one(fr[0], lds0, std::integral_constant<int, 0>{}, x); });
     for (int t = t0; t < t1; ++t) {
-        // stage t has landed once at most the copies of the AHEAD - 1 younger stages are outstanding; past the barrier it
-        // has for every wave, and every wave has left the slot of stage t - 1
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((AHEAD - 1) * (CA + CB)) : "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        const int next = slot + AHEAD >= G::STAGES ? slot + AHEAD - G::STAGES : slot + AHEAD;
-        copy_stage(t + AHEAD, next);
         const unsigned base = lds0 + slot * G::STAGE_BYTES;
-        read_step(fr[0], base, std::integral_constant<int, 0>{});
+        const int next = slot + 1 == G::STAGES ? 0 : slot + 1, before = slot ? slot - 1 : G::STAGES - 1;
+        const unsigned next_base = lds0 + next * G::STAGE_BYTES;
         tok_static_for<KS>([&](auto s) {
             constexpr int S = decltype(s)::value;
-            if constexpr (S + 1 < KS) {
-                read_step(fr[(S + 1) & 1], base, std::integral_constant<int, S + 1>{});
-                settle(fr[S & 1], std::integral_constant<int, STEP_READS>{});
-            } else {
-                settle(fr[S & 1], std::integral_constant<int, 0>{});
+            constexpr bool LAST = S + 1 == KS;
+            Frags &f = fr[S & 1];
+            settle(f);
+            if constexpr (LAST) {
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"((G::STAGES - 2) * (CA + CB)) : "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
             }
-            multiply(fr[S & 1]);
+            __builtin_amdgcn_sched_barrier(0);
+            constexpr int SHARE0 = LAST ? 0 : FIRST_PART, SHARE1 = LAST ? FIRST_PART : (S == 0 ? CA + CB : FIRST_PART);
+            tok_static_for<MFMAS>([&](auto mm) {
+                constexpr int M = decltype(mm)::value;
+                tok_mfma<T>(f.b[M % NT], f.a[M / NT], acc[M / NT][M % NT]);
+                if constexpr (M < READ_SLOTS) {
+                    constexpr int X0 = READS * M / READ_SLOTS, X1 = READS * (M + 1) / READ_SLOTS;
+                    tok_static_for<X1 - X0>([&](auto x) {
+                        // (behind the last stage: zeros that nothing uses, but the slot is there)
+                        read_one(fr[(S + 1) & 1], LAST ? next_base : base, std::integral_constant<int, LAST ? 0 : S + 1>{},
+                                 std::integral_constant<int, X0 + decltype(x)::value>{});
+                    });
+                }
+                if constexpr (M >= COPY_SLOT) {
+                    constexpr int A0 = SHARE0 + (SHARE1 - SHARE0) * (M - COPY_SLOT) / (MFMAS - COPY_SLOT);
+                    constexpr int A1 = SHARE0 + (SHARE1 - SHARE0) * (M + 1 - COPY_SLOT) / (MFMAS - COPY_SLOT);
+                    tok_static_for<A1 - A0>([&](auto x) {
+                        copy_one(LAST ? slot : before, std::integral_constant<int, A0 + decltype(x)::value>{});
+                    });
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            });
         });
-        slot = slot + 1 == G::STAGES ? 0 : slot + 1;
+        slot = next;
     }
-    // no copy may still be on its way into this workgroup's LDS when it ends
+    // the reads behind the last stage return into registers that are still theirs, and no copy may be on its way into this
+    // workgroup's LDS when it is used again or ends
+    settle(fr[0]);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 
-    // Accumulator element e of a fragment: m = lane & 31, n = (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5).
+    // Accumulator element e of a fragment: m = lane & 31, n = (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5).  Stored from there
+    // a wave instruction would touch 32 rows, 16 bytes each; instead the wave's results turn in the LDS, TURN fragments of 32
+    // rows at a time (fp32, 16-byte chunk c of row m at c ^ (m mod chunks): both directions use all banks), and every lane
+    // goes on with eight consecutive columns of a row, so that memory sees whole 128-byte lines.  The rows are a loop, with
+    // the activation chosen outside of it: unrolled over rows and activations the code is larger than the instruction cache
+    // and its fetch took longer than the main loop (training step of 16384 x 1024 x 4096: 354 + 310 us for the two products
+    // with an activation).
     constexpr bool EXACT = sizeof(T) == 4;
-    const int half4 = 4 * (lane >> 5);
+    constexpr int CHUNKS = NT * 8;                          // of 4 columns
+    constexpr int COLS = EPI == TOK_EPI_GLU ? NT * 16 : NT * 32;
+    constexpr int LANES = COLS / 8, ROWS = 64 / LANES;      // lanes of a row, rows of an instruction
+    unsigned char *const turn = smem + wave * (G::TURN * 32 * G::TURN_ROW);
+    const int col = (lane % LANES) * 8;
+    const int n = n0 + wn * COLS + col;
+    auto turned = [&](int r, int chunk) -> tok_f32x4 {
+        return *reinterpret_cast<const tok_f32x4 *>(turn + (r * CHUNKS + (chunk ^ (r % CHUNKS))) * 16);
+    };
+    // results without an activation go out 16 bytes at a time where their rows allow it
+    constexpr int NARROW = 0, WIDE = 1;
+    const bool wide = (job.N & 7) == 0 && (EPI == TOK_EPI_PART || ((job.c_ld & 7) == 0 && ((size_t)job.c & 15) == 0));
+    float bias[8], bias2[8];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const long long m = m0 + (wm * MT + i) * 32 + (lane & 31);
-        if (m >= job.M) continue;
-        if constexpr (EPI == TOK_EPI_GLU) {
-            static_assert(NT == 2, "a wave holds the gate and the up columns of 32 hidden channels");
-            const int nb = n0 + wn * 32 + half4;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int n = nb + 8 * q;
-                if (n >= p.h_ld) continue;
-                float g4[4], u4[4], h4[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    // columns past the hidden width (up to the padded row) have zero products and no bias: they store zeros
-                    g4[j] = acc[i][0][4 * q + j], u4[j] = acc[i][NT - 1][4 * q + j];
-                    if (job.bias && n + j < job.N) g4[j] += (float)((const T *)job.bias)[n + j];
-                    if (p.bias_up && n + j < job.N) u4[j] += (float)((const T *)p.bias_up)[n + j];
-                    h4[j] = tok_act<EXACT>(p.act, g4[j]) * u4[j];
-                }
+    for (int j = 0; j < 8; ++j) {
+        // columns past the hidden width (up to the padded row) have zero products and no bias: they store zeros
+        bias[j] = (EPI == TOK_EPI_GLU || EPI == TOK_EPI_STORE) && job.bias && n + j < job.N ? (float)((const T *)job.bias)[n + j] : 0.f;
+        bias2[j] = EPI == TOK_EPI_GLU && p.bias_up && n + j < job.N ? (float)((const T *)p.bias_up)[n + j] : 0.f;
+    }
+    const bool in_n = n < (EPI == TOK_EPI_GLU || EPI == TOK_EPI_GLU_GRAD ? p.h_ld : (long long)job.N);
+    // rows [r of the turned fragments], all of this lane's columns
+    auto finish = [&](auto kind, long long m_first) {
+        constexpr int KIND = decltype(kind)::value;
+#pragma unroll 2
+        for (int r = lane / LANES; r < G::TURN * 32; r += ROWS) {
+            const long long m = m_first + r;
+            const tok_f32x4 lo = turned(r, col / 4), hi = turned(r, col / 4 + 1);
+            float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            if (m >= job.M || !in_n) continue;
+            if constexpr (EPI == TOK_EPI_GLU) {
+                const tok_f32x4 lo2 = turned(r, NT * 4 + col / 4), hi2 = turned(r, NT * 4 + col / 4 + 1);
+                float w[8] = {lo2[0], lo2[1], lo2[2], lo2[3], hi2[0], hi2[1], hi2[2], hi2[3]}, h[8];
                 const long long at = m * p.h_ld + n;
-                tok_store4<T>((T *)p.h + at, h4);
                 if (p.g) {
-                    tok_store4<T>((T *)p.g + at, g4);
-                    tok_store4<T>((T *)p.u + at, u4);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float up = w[j] + bias2[j];
+                        float da;
+                        tok_act_grad<EXACT, KIND>(v[j] + bias[j], v[j], da);
+                        h[j] = v[j] * up, w[j] = up * da;
+                    }
+                    tok_store8<T>((T *)p.g + at, v);
+                    tok_store8<T>((T *)p.u + at, w);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) h[j] = tok_act<EXACT, KIND>(v[j] + bias[j]) * (w[j] + bias2[j]);
+                }
+                tok_store8<T>((T *)p.h + at, h);
+            } else if constexpr (EPI == TOK_EPI_GLU_GRAD) {
+                const long long at = m * p.h_ld + n;
+                float a[8], d[8];
+                tok_load8<T>((const T *)p.sg + at, a);
+                tok_load8<T>((const T *)p.su + at, d);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) d[j] *= v[j], a[j] *= v[j];
+                tok_store8<T>((T *)p.g + at, d);
+                tok_store8<T>((T *)p.u + at, a);
+            } else if constexpr (EPI == TOK_EPI_PART) {
+                float *part = job.part + ((size_t)split * job.M + m) * job.N + n;
+                if constexpr (KIND == WIDE) {
+                    tok_store8<float>(part, v);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (n + j < job.N) part[j] = v[j];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] += bias[j];
+                T *c = (T *)job.c + m * job.c_ld + n;
+                if constexpr (KIND == WIDE) {
+                    tok_store8<T>(c, v);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (n + j < job.N) c[j] = (T)v[j];
                 }
             }
-        } else {
+        }
+    };
 #pragma unroll
-            for (int jn2 = 0; jn2 < NT; ++jn2) {
-                const int nb = n0 + (wn * NT + jn2) * 32 + half4;
+    for (int i0 = 0; i0 < MT; i0 += G::TURN) {
+        asm volatile("" ::: "memory");                      // (the lanes of a wave read what others of them wrote, in order)
+#pragma unroll
+        for (int i = 0; i < G::TURN; ++i) {
+            const int r0 = i * 32 + (lane & 31);
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const int n = nb + 8 * q;
-                    float v[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j] = acc[i][jn2][4 * q + j];
-                    if constexpr (EPI == TOK_EPI_GLU_GRAD) {
-                        if (n >= p.h_ld) continue;
-                        const long long at = m * p.h_ld + n;
-                        float g4[4], u4[4], dg[4], du[4];
-                        tok_load4<T>((const T *)p.sg + at, g4);
-                        tok_load4<T>((const T *)p.su + at, u4);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            float act, da;
-                            tok_act_grad<EXACT>(p.act, g4[j], act, da);
-                            dg[j] = v[j] * u4[j] * da, du[j] = v[j] * act;
-                        }
-                        tok_store4<T>((T *)p.g + at, dg);
-                        tok_store4<T>((T *)p.u + at, du);
-                    } else if constexpr (EPI == TOK_EPI_PART) {
-                        if (n >= job.N) continue;
-                        float *part = job.part + ((size_t)split * job.M + m) * job.N + n;
-                        if ((job.N & 3) == 0) {
-                            tok_store4<float>(part, v);
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                if (n + j < job.N) part[j] = v[j];
-                        }
-                    } else {
-                        if (n >= job.N) continue;
-                        if (job.bias) {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                if (n + j < job.N) v[j] += (float)((const T *)job.bias)[n + j];
-                        }
-                        T *c = (T *)job.c + m * job.c_ld + n;
-                        if ((job.N & 3) == 0 && (job.c_ld & 3) == 0 && ((size_t)job.c & 15) == 0) {
-                            tok_store4<T>(c, v);
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                if (n + j < job.N) c[j] = (T)v[j];
-                        }
-                    }
+                    const int chunk = j * 8 + q * 2 + (lane >> 5);
+                    const tok_f32x16 &a = acc[i0 + i][j];
+                    *reinterpret_cast<tok_f32x4 *>(turn + (r0 * CHUNKS + (chunk ^ (r0 % CHUNKS))) * 16) =
+                        tok_f32x4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
                 }
-            }
+        }
+        asm volatile("" ::: "memory");
+        const long long m_first = m0 + (wm * MT + i0) * 32;
+        if constexpr (EPI == TOK_EPI_GLU) {
+            if (p.act == SR355_ACT_SILU) finish(std::integral_constant<int, SR355_ACT_SILU>{}, m_first);
+            else if (p.act == SR355_ACT_GELU) finish(std::integral_constant<int, SR355_ACT_GELU>{}, m_first);
+            else if (p.act == SR355_ACT_RELU) finish(std::integral_constant<int, SR355_ACT_RELU>{}, m_first);
+            else finish(std::integral_constant<int, SR355_ACT_SIGMOID>{}, m_first);
+        } else {
+            if (EPI == TOK_EPI_GLU_GRAD || wide) finish(std::integral_constant<int, WIDE>{}, m_first);
+            else finish(std::integral_constant<int, NARROW>{}, m_first);
         }
     }
 }

@@ -311,15 +311,16 @@ def ffn_bounds(x, dy, ws, bs, act, u):
     e_h = e_a * uu.abs() + a.abs() * e_u + 2 * u * h.abs()
     y = h @ T(wd) + bd
     t_y = e_h @ T(wd.abs()) + (f + 4) * B * (h.abs() @ T(wd.abs()) + bd.abs()) + u * y.abs()
-    # the backward pass reads g and u as they are held: rounded to the type
-    e_gs, e_us = e_g + 1.01 * u * g.abs(), e_u + 1.01 * u * uu.abs()
+    # the backward pass multiplies dh with act(g) and u act'(g), which are held rounded to the type: |a~ - a| <= e_a + u |a|
+    # and, with d = u act'(g), |d~ - d| <= (e_u |act'| + |u| e_act') (1 + ..) + u |d|
     e_dh = (c + 4) * B * (dyd.abs() @ wd.abs())
-    e_da = 0.8 * e_gs + fn * (1 + da.abs())
+    e_da = 0.8 * e_g + fn * (1 + da.abs())
     if act == "relu":
-        e_da = (g.abs() <= 2 * e_gs).double()
-    e_as = 1.13 * e_gs + fn * a.abs()
+        e_da = (g.abs() <= 2 * e_g).double()
+    e_as = e_a + 1.01 * u * a.abs()
+    e_d = e_u * (da.abs() + e_da) + uu.abs() * e_da + 1.01 * u * (uu * da).abs()
     grow = 1.01
-    e_dg = grow * (e_dh * (uu * da).abs() + dh.abs() * (e_us * (da.abs() + e_da) + uu.abs() * e_da) + 4 * B * dg.abs()) + 1.01 * u * dg.abs()
+    e_dg = grow * (e_dh * (uu * da).abs() + dh.abs() * e_d + 4 * B * dg.abs()) + 1.01 * u * dg.abs()
     e_du = grow * (e_dh * a.abs() + dh.abs() * e_as + 4 * B * du.abs()) + 1.01 * u * du.abs()
     dx = dg @ wg + du @ wu
     t_dx = e_dg @ wg.abs() + e_du @ wu.abs() + (2 * f + 4) * B * (dg.abs() @ wg.abs() + du.abs() @ wu.abs()) + u * dx.abs()
