@@ -13,7 +13,7 @@
 //
 // Operands are read 16 bytes at a time.  What does not allow that (a width, stride or pointer that is no multiple of 16
 // bytes) is first copied into padded rows of the workspace, one launch for all of them.
-#include "token_gemm.h"
+#include "token_rows.h"
 
 namespace sr355 {
 
@@ -24,10 +24,7 @@ namespace {
 // more latency than two of 128 (443 against 472 us for the three weight gradients of 16384 x 1024 x 4096).
 typedef TokTile<256, 256, 2, 4, 128, 2> Tile256;
 typedef TokTile<256, 256, 2, 4, 64, 5> TileWgrad;
-#ifndef T128
-#define T128 128, 128, 2, 2, 128, 2
-#endif
-typedef TokTile<T128> Tile128;
+typedef TokTile<128, 128, 2, 2, 128, 2> Tile128;
 constexpr int N_CU = 256;
 
 struct PadJob {
@@ -62,6 +59,8 @@ struct ReduceArgs {
     void *out[3];
     long long n[3];
     int splits;
+    const void *bias;        // of columns (job 0), may be null
+    int cols;
 };
 template <typename T>
 __global__ __launch_bounds__(256) void reduce_splits_kernel(ReduceArgs a) {
@@ -78,6 +77,10 @@ __global__ __launch_bounds__(256) void reduce_splits_kernel(ReduceArgs a) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[j] += t[j];
             }
+            if (a.bias) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] += (float)((const T *)a.bias)[(i + j) % a.cols];
+            }
             T o[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[j] = (T)v[j];
@@ -85,6 +88,7 @@ __global__ __launch_bounds__(256) void reduce_splits_kernel(ReduceArgs a) {
         } else {
             for (int j = 0; j < 4 && i + j < n; ++j) {
                 for (int s = 0; s < a.splits; ++s) v[j] += part[(size_t)s * n + i + j];
+                if (a.bias) v[j] += (float)((const T *)a.bias)[(i + j) % a.cols];
                 out[i + j] = (T)v[j];
             }
         }
@@ -171,6 +175,64 @@ int gemm_pick(TokGemmArgs &g, const char *what, hipStream_t stream) {
     return gemm_launch<T, Tile128, A_RC, B_RC, EPI>(g, what, stream);
 }
 
+// Into how many parts the sum over k of a few tiles is split: the number that takes least, by the rounds of the chip
+// (`slots` workgroups at a time) and the partials' way through memory (8 bytes an element and part at 5 TB/s, and a launch).
+// Microseconds of a stage, with as many workgroups per CU as fit: what the kernels take on full rounds.
+struct Splits {
+    int n, stages;      // parts, stages of a part
+};
+Splits pick_splits(long long tiles, int slots, long long stages, double elements, double stage_us) {
+    if (stages < 1) stages = 1;
+    Splits best = {1, (int)stages};
+    double least = 1e30;
+    for (long long s = 1; s <= 64 && s <= (stages + 3) / 4; ++s) {
+        const long long per = tok_cdiv(stages, s), n = tok_cdiv(stages, per);
+        const double us = (double)tok_cdiv(tiles * n, slots) * per * stage_us + (n > 1 ? 4.0 + 8e-6 / 5.0 * n * elements : 0.0);
+        if (us < least) least = us, best = {(int)n, (int)per};
+    }
+    return best;
+}
+template <typename G>
+double stage_us(int dtype) {
+    // MFMA cycles of a stage's workgroups on a CU (32 a 32 x 32 x 16, 64 a 32 x 32 x 2) at 2 GHz and 70 % of the pipes
+    const double wgs = G::LDS_BYTES > 80 * 1024 ? 1 : 2;
+    const double mfma = (double)G::MT * G::NT * G::KS * (dtype == SR355_DTYPE_F32 ? 4 * 64 : 32) * (G::WAVES / 4);
+    return mfma * wgs / 2000.0 / 0.7;
+}
+
+// A product of rows and weights, split over k where its tiles are few; `parts` null: not split.
+bool product_is_big(long long rows, int n) { return tok_cdiv(rows, Tile256::BM) * tok_cdiv(n, Tile256::BN) >= N_CU; }
+Splits product_splits(long long rows, int n, int k, int sections, int dtype) {
+    if (product_is_big(rows, n)) return {1, 0};
+    const long long tiles = tok_cdiv(rows, Tile128::BM) * tok_cdiv(n, Tile128::BN);
+    const long long stages = tok_cdiv(k, Tile128::KB / (long long)tok_type_bytes(dtype)) * sections;
+    return pick_splits(tiles, 2 * N_CU, stages, (double)rows * n, stage_us<Tile128>(dtype));
+}
+
+template <typename T>
+int reduce_launch(const ReduceArgs &r, int n_jobs, const char *what, hipStream_t stream) {
+    long long most = 0;
+    for (int i = 0; i < n_jobs; ++i)
+        if (r.n[i] > most) most = r.n[i];
+    const long long wgs = tok_cdiv(most, 1024);
+    hipLaunchKernelGGL((reduce_splits_kernel<T>), dim3((unsigned)(wgs > 2048 ? 2048 : wgs), n_jobs), dim3(256), 0, stream, r);
+    return check_hip(hipGetLastError(), what);
+}
+
+template <typename T, bool B_RC>
+int product_launch(TokGemmArgs &g, const Splits &split, float *parts, const char *what, hipStream_t stream) {
+    if (!parts) return gemm_pick<T, false, B_RC, TOK_EPI_STORE>(g, what, stream);
+    TokJob &j = g.job[0];
+    g.splits = split.n, g.split_stages = split.stages;
+    j.part = parts;
+    set_tiles<Tile128>(g, false);
+    const int rc = gemm_launch<T, Tile128, false, B_RC, TOK_EPI_PART>(g, what, stream);
+    if (rc != SR355_OK) return rc;
+    ReduceArgs r = {};
+    r.part[0] = parts, r.out[0] = j.c, r.n[0] = (long long)j.M * j.N, r.splits = split.n, r.bias = j.bias, r.cols = j.N;
+    return reduce_launch<T>(r, 1, what, stream);
+}
+
 // ---- the plan of a call: what is copied, where things lie in the workspace --------------------------------------------
 struct Operand {
     const void *p;
@@ -220,9 +282,14 @@ size_t hidden_bytes(const sr355_ffn_args *a) {
     return ((size_t)a->rows * hidden_ld(a) * tok_type_bytes(a->dtype) + 255) & ~(size_t)255;
 }
 
+// up to so many rows the kernels of token_rows.h: reading the weights bounds them
+constexpr int FEW_ROWS = 64;
+
 struct ForwardPlan : Plan {
     Operand x, wg, wu, wd;
     void *g, *u, *h;
+    Splits down;
+    float *parts = nullptr;
 
     ForwardPlan(const sr355_ffn_args *a, unsigned char *ws) {
         base = ws;
@@ -236,14 +303,19 @@ struct ForwardPlan : Plan {
         } else {
             g = u = nullptr, h = take(hidden_bytes(a));
         }
+        if (a->rows > FEW_ROWS) {
+            down = product_splits(a->rows, a->channels, a->hidden, 1, a->dtype);
+            if (down.n > 1) parts = (float *)take((size_t)down.n * a->rows * a->channels * sizeof(float));
+            split = down.n > 1;
+        }
     }
+    bool split = false;
 };
 
-// Workgroups of the weight gradients: k is the rows, so a few tiles with a long k are split until the chip is full, with
-// at least eight stages (512 rows) a split.
+// The weight gradients: k is the rows.
 struct WgradShape {
     bool big;
-    int splits, split_stages;
+    Splits split;
 };
 template <typename G>
 long long wgrad_tiles(const sr355_ffn_args *a) {
@@ -251,25 +323,24 @@ long long wgrad_tiles(const sr355_ffn_args *a) {
     const long long c_f = tok_cdiv(a->channels, G::BM) * tok_cdiv(a->hidden, G::BN);
     return (a->dw_gate_dev ? f_c : 0) + (a->dw_up_dev ? f_c : 0) + (a->dw_down_dev ? c_f : 0);
 }
+template <typename G>
+Splits wgrad_splits(const sr355_ffn_args *a, int slots) {
+    const int mats = (a->dw_gate_dev != nullptr) + (a->dw_up_dev != nullptr) + (a->dw_down_dev != nullptr);
+    return pick_splits(wgrad_tiles<G>(a), slots, tok_cdiv(a->rows, G::KB / (long long)tok_type_bytes(a->dtype)),
+                       (double)mats * a->hidden * a->channels, stage_us<G>(a->dtype));
+}
 WgradShape wgrad_shape(const sr355_ffn_args *a) {
-    WgradShape w;
-    w.big = wgrad_tiles<TileWgrad>(a) >= N_CU / 4;
-    const long long stages = tok_cdiv(a->rows, (w.big ? TileWgrad::KB : Tile128::KB) / (long long)tok_type_bytes(a->dtype));
-    const long long tiles = w.big ? wgrad_tiles<TileWgrad>(a) : wgrad_tiles<Tile128>(a);
-    const long long want = tok_cdiv(w.big ? N_CU : 2 * N_CU, tiles < 1 ? 1 : tiles);
-    long long splits = stages / 8 < want ? stages / 8 : want;
-    if (splits < 1) splits = 1;
-    w.split_stages = (int)tok_cdiv(stages < 1 ? 1 : stages, splits);
-    w.splits = (int)tok_cdiv(stages < 1 ? 1 : stages, w.split_stages);
-    return w;
+    if (wgrad_tiles<TileWgrad>(a) >= N_CU / 4) return {true, wgrad_splits<TileWgrad>(a, N_CU)};
+    return {false, wgrad_splits<Tile128>(a, 2 * N_CU)};
 }
 
 struct BackwardPlan : Plan {
     Operand x, dy, wg, wu, wd;
     void *dg, *du;
     const void *g, *u, *h;
-    float *parts, *col_parts;
+    float *parts, *col_parts, *dx_parts;
     WgradShape wgrad;
+    Splits dx;
     bool need_hidden;
 
     BackwardPlan(const sr355_ffn_args *a, unsigned char *ws) {
@@ -290,8 +361,11 @@ struct BackwardPlan : Plan {
         du = need_hidden ? take(hidden_bytes(a)) : nullptr;
         wgrad = wgrad_shape(a);
         const size_t mats = (a->dw_gate_dev != nullptr) + (a->dw_up_dev != nullptr) + (a->dw_down_dev != nullptr);
-        parts = mats && wgrad.splits > 1
-                    ? (float *)take(mats * wgrad.splits * (size_t)a->hidden * a->channels * sizeof(float)) : nullptr;
+        parts = mats && wgrad.split.n > 1
+                    ? (float *)take(mats * wgrad.split.n * (size_t)a->hidden * a->channels * sizeof(float)) : nullptr;
+        dx = {1, 0};
+        if (a->dx_dev && a->rows > 0) dx = product_splits(a->rows, a->channels, a->hidden, 2, a->dtype);
+        dx_parts = dx.n > 1 ? (float *)take((size_t)dx.n * a->rows * a->channels * sizeof(float)) : nullptr;
         const bool cols = a->db_gate_dev || a->db_up_dev || a->db_down_dev;
         col_parts = cols ? (float *)take((size_t)COL_PARTS * (2 * hidden_ld(a) + dy.ld) * sizeof(float)) : nullptr;
     }
@@ -311,11 +385,43 @@ bool ffn_args_ok(const char *who, const sr355_ffn_args *a, bool backward) {
     return true;
 }
 
+template <typename T, int TG, bool GLU, int WAVES>
+int few_rows(TokRowsArgs a, const char *what, hipStream_t stream) {
+    a.channels = 16;
+    while (a.channels > 4 && tok_cdiv(a.n_store, a.channels) < N_CU) a.channels /= 2;
+    hipLaunchKernelGGL((tok_rows_kernel<T, TG, GLU, WAVES>), dim3((unsigned)tok_cdiv(a.n_store, a.channels)), dim3(64 * WAVES), 0, stream, a);
+    return check_hip(hipGetLastError(), what);
+}
+template <typename T, int TG>
+int few_rows_both(const TokRowsArgs &glu, const TokRowsArgs &down, hipStream_t stream) {
+    const int rc = few_rows<T, TG, true, TG == 4 ? 4 : 8>(glu, "gated_ffn gate / up launch", stream);
+    return rc != SR355_OK ? rc : few_rows<T, TG, false, TG == 4 ? 8 : 16>(down, "gated_ffn down launch", stream);
+}
+
+template <typename T>
+int ffn_forward_few(const sr355_ffn_args *a, const ForwardPlan &p, hipStream_t stream) {
+    TokRowsArgs g = {};
+    g.x = (const unsigned char *)p.x.p, g.x_ld = p.x.ld * sizeof(T);
+    g.w = (const unsigned char *)p.wg.p, g.w2 = (const unsigned char *)p.wu.p, g.w_ld = p.wg.ld * sizeof(T);
+    g.rows = (int)a->rows, g.N = a->hidden, g.k_bytes = (int)(a->channels * sizeof(T));
+    g.bias = a->b_gate_dev, g.bias2 = a->b_up_dev, g.act = a->activation;
+    g.out = p.h, g.kept_a = p.g, g.kept_d = p.u, g.out_ld = hidden_ld(a), g.n_store = (int)hidden_ld(a);
+    TokRowsArgs d = {};
+    d.x = (const unsigned char *)p.h, d.x_ld = hidden_ld(a) * sizeof(T);
+    d.w = (const unsigned char *)p.wd.p, d.w_ld = p.wd.ld * sizeof(T);
+    d.rows = (int)a->rows, d.N = a->channels, d.k_bytes = (int)(a->hidden * sizeof(T)), d.bias = a->b_down_dev;
+    d.out = a->y_dev, d.out_ld = a->channels, d.n_store = a->channels;
+    if (a->rows <= 16) return few_rows_both<T, 1>(g, d, stream);
+    if (a->rows <= 32) return few_rows_both<T, 2>(g, d, stream);
+    return few_rows_both<T, 4>(g, d, stream);
+}
+
 template <typename T>
 int ffn_forward(const sr355_ffn_args *a, hipStream_t stream) {
     ForwardPlan p(a, (unsigned char *)a->workspace_dev);
     int rc = run_pads<T>(p, stream);
     if (rc != SR355_OK) return rc;
+    if (a->rows <= FEW_ROWS) return ffn_forward_few<T>(a, p, stream);
     TokGemmArgs g = {};
     g.n_jobs = 1, g.sections = 1, g.act = a->activation, g.K = a->channels;
     TokJob &j = g.job[0];
@@ -331,13 +437,13 @@ int ffn_forward(const sr355_ffn_args *a, hipStream_t stream) {
     k.a[0] = (const unsigned char *)p.h, k.a_ld = hidden_ld(a) * sizeof(T);
     k.b[0] = (const unsigned char *)p.wd.p, k.b_ld = p.wd.ld * sizeof(T);
     k.M = (int)a->rows, k.N = a->channels, k.bias = a->b_down_dev, k.c = a->y_dev, k.c_ld = a->channels;
-    return gemm_pick<T, false, false, TOK_EPI_STORE>(d, "gated_ffn down launch", stream);
+    return product_launch<T, false>(d, p.down, p.split ? p.parts : nullptr, "gated_ffn down launch", stream);
 }
 
 template <typename T>
 int ffn_wgrad(const sr355_ffn_args *a, const BackwardPlan &p, hipStream_t stream) {
     TokGemmArgs g = {};
-    g.sections = 1, g.K = (int)a->rows, g.splits = p.wgrad.splits, g.split_stages = p.wgrad.split_stages;
+    g.sections = 1, g.K = (int)a->rows, g.splits = p.wgrad.split.n, g.split_stages = p.wgrad.split.stages;
     ReduceArgs r = {};
     float *parts = p.parts;
     const size_t n = (size_t)a->hidden * a->channels;
@@ -348,7 +454,7 @@ int ffn_wgrad(const sr355_ffn_args *a, const BackwardPlan &p, hipStream_t stream
         j.b[0] = (const unsigned char *)q, j.b_ld = q_ld * sizeof(T);
         j.M = M, j.N = N, j.c = out, j.c_ld = N, j.part = parts;
         r.part[g.n_jobs] = parts, r.out[g.n_jobs] = out, r.n[g.n_jobs] = (long long)n;
-        if (parts) parts += p.wgrad.splits * n;
+        if (parts) parts += p.wgrad.split.n * n;
         ++g.n_jobs;
     };
     add(p.dg, hidden_ld(a), p.x.p, p.x.ld, a->hidden, a->channels, a->dw_gate_dev);
@@ -367,10 +473,8 @@ int ffn_wgrad(const sr355_ffn_args *a, const BackwardPlan &p, hipStream_t stream
                      : gemm_launch<T, Tile128, true, true, TOK_EPI_STORE>(g, what, stream);
     }
     if (rc != SR355_OK || !p.parts) return rc;
-    r.splits = p.wgrad.splits;
-    const long long wgs = tok_cdiv((long long)n, 1024);
-    hipLaunchKernelGGL((reduce_splits_kernel<T>), dim3((unsigned)(wgs > 2048 ? 2048 : wgs), g.n_jobs), dim3(256), 0, stream, r);
-    return check_hip(hipGetLastError(), "gated_ffn weight gradient reduction launch");
+    r.splits = p.wgrad.split.n;
+    return reduce_launch<T>(r, g.n_jobs, "gated_ffn weight gradient reduction launch", stream);
 }
 
 template <typename T>
@@ -396,7 +500,7 @@ int ffn_backward(const sr355_ffn_args *a, hipStream_t stream) {
         j.a[0] = (const unsigned char *)p.dg, j.a[1] = (const unsigned char *)p.du, j.a_ld = hidden_ld(a) * sizeof(T);
         j.b[0] = (const unsigned char *)p.wg.p, j.b[1] = (const unsigned char *)p.wu.p, j.b_ld = p.wg.ld * sizeof(T);
         j.M = (int)a->rows, j.N = a->channels, j.c = a->dx_dev, j.c_ld = a->channels;
-        rc = gemm_pick<T, false, true, TOK_EPI_STORE>(g, "gated_ffn data gradient launch", stream);
+        rc = product_launch<T, true>(g, p.dx, p.dx_parts, "gated_ffn data gradient launch", stream);
         if (rc != SR355_OK) return rc;
     }
     rc = ffn_wgrad<T>(a, p, stream);

@@ -263,11 +263,12 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
     const long long a_step = A_RC ? BK * job.a_ld : G::KB, b_step = B_RC ? BK * job.b_ld : G::KB;
     const long long a_corner = A_RC ? m0 * (long long)sizeof(T) : m0 * job.a_ld;
     const long long b_corner = B_RC ? n0 * (long long)sizeof(T) : n0 * job.b_ld;
-    const unsigned char *pa = job.a[0] + a_corner + t0 * a_step, *pb = job.b[0] + b_corner + t0 * b_step;
+    const int sec0 = EPI == TOK_EPI_PART && t0 >= n_stage ? 1 : 0, in_sec = t0 - sec0 * n_stage;   // the section of the first stage
+    const unsigned char *pa = job.a[sec0] + a_corner + in_sec * a_step, *pb = job.b[sec0] + b_corner + in_sec * b_step;
     const long long up_off = job.b[1] - job.b[0];          // GLU: both weights' rows are of one stride
     const unsigned char *const pa1 = job.a[1] + a_corner, *const pb1 = job.b[1] + b_corner;
-    const int sections = EPI == TOK_EPI_STORE ? p.sections : 1;
-    int copy_t = t0, left = p.K - t0 * BK;
+    const int sections = EPI == TOK_EPI_STORE || EPI == TOK_EPI_PART ? p.sections : 1;
+    int copy_t = t0, left = p.K - in_sec * BK;
     const int K = p.K;
     // Copy I of this wave's CA + CB copies of the stage.  Past the last stage it copies zeros, so that the counted waits always
     // see the same number of copies.
