@@ -14,54 +14,15 @@ from typing import Optional
 
 import torch
 from torch import Tensor, nn
-from torch.autograd.function import once_differentiable
 
 from . import token_ops as ops
-
-
-def _recorded(*ts: Optional[Tensor]) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: float) -> Tensor:
-        y, stats = ops.layer_norm_fwd_now(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, stats)
-        ctx.param_dtype = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy: Tensor):
-        x, weight, stats = ctx.saved_tensors
-        need = list(ctx.needs_input_grad[:3])
-        grads = ops.layer_norm_bwd_now(dy, x, weight, stats, ctx.param_dtype, need)
-        return (*(g if n else None for g, n in zip(grads, need)), None)
 
 
 def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5) -> Tensor:
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension of ``x``.  ``weight`` and ``bias``, ``[C]``,
     are of x's type or float32 (both of one type), and so are their gradients.  A row of one channel or of equal channels
     gives ``bias``."""
-    if _recorded(x, weight, bias):
-        return _LayerNorm.apply(x, weight, bias, eps)
-    return ops.layer_norm_fwd_now(x, weight, bias, eps, False)[0]
-
-
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x: Tensor, p: float, rng: Tensor, site: int, residual: Optional[Tensor]) -> Tensor:
-        ctx.save_for_backward(rng)
-        ctx.p, ctx.site = p, site
-        return ops.dropout_now(x, residual, p, rng, site)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy: Tensor):
-        (rng,) = ctx.saved_tensors
-        dx = ops.dropout_now(dy, None, ctx.p, rng, ctx.site) if ctx.needs_input_grad[0] else None
-        return dx, None, None, None, dy if ctx.needs_input_grad[4] else None
+    return (ops._binding or ops.binding()).layer_norm(x, weight, bias, eps)
 
 
 def dropout(x: Tensor, p: float, rng: Tensor, site: int = 0, residual: Optional[Tensor] = None) -> Tensor:
@@ -74,26 +35,7 @@ def dropout(x: Tensor, p: float, rng: Tensor, site: int = 0, residual: Optional[
     it runs, so a captured graph's replays drop what the words say then; changing them in place between a call and its
     backward pass is an error that autograd reports.  ``p`` counts in steps of 2^-16 and the scale is that of the nearest
     step; a dropped infinity or NaN is dropped."""
-    if _recorded(x, residual):
-        return _Dropout.apply(x, p, rng, site, residual)
-    return ops.dropout_now(x, residual, p, rng, site)
-
-
-class _GatedFfn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, b_gate: Optional[Tensor],
-                b_up: Optional[Tensor], b_down: Optional[Tensor], activation: int) -> Tensor:
-        y, saved = ops.gated_ffn_fwd_now(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation, True)
-        ctx.save_for_backward(x, w_gate, w_up, w_down, saved)
-        ctx.activation = activation
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy: Tensor):
-        need = list(ctx.needs_input_grad[:7])
-        grads = ops.gated_ffn_bwd_now(dy, *ctx.saved_tensors, ctx.activation, need)
-        return (*(g if n else None for g, n in zip(grads, need)), None)
+    return (ops._binding or ops.binding()).dropout(x, p, rng, site, residual)
 
 
 def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, b_gate: Optional[Tensor] = None,
@@ -104,10 +46,7 @@ def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, b_gate: O
     between the launches.  A call that autograd records keeps three rows of F hidden channels per row of x."""
     if activation not in ops.ACTIVATIONS:
         raise RuntimeError(f"gated_ffn: activation must be one of {', '.join(ops.ACTIVATIONS)}, got {activation!r}")
-    code = ops.ACTIVATIONS[activation]
-    if _recorded(x, w_gate, w_up, w_down, b_gate, b_up, b_down):
-        return _GatedFfn.apply(x, w_gate, w_up, w_down, b_gate, b_up, b_down, code)
-    return ops.gated_ffn_fwd_now(x, w_gate, w_up, w_down, b_gate, b_up, b_down, code, False)[0]
+    return (ops._binding or ops.binding()).gated_ffn(x, w_gate, w_up, w_down, b_gate, b_up, b_down, ops.ACTIVATIONS[activation])
 
 
 def rows_from_blocked(x: Tensor, channels: int) -> Tensor:
