@@ -13,6 +13,7 @@
 //
 // Operands are read 16 bytes at a time.  What does not allow that (a width, stride or pointer that is no multiple of 16
 // bytes) is first copied into padded rows of the workspace, one launch for all of them.
+#include "token_narrow.h"
 #include "token_rows.h"
 
 namespace sr355 {
@@ -34,7 +35,7 @@ struct PadJob {
     int cols;
 };
 struct PadArgs {
-    PadJob job[5];
+    PadJob job[6];
 };
 // rows of `cols` elements into rows of dst_ld (a multiple of a unit), zeros behind
 template <typename T>
@@ -282,12 +283,19 @@ size_t hidden_bytes(const sr355_ffn_args *a) {
     return ((size_t)a->rows * hidden_ld(a) * tok_type_bytes(a->dtype) + 255) & ~(size_t)255;
 }
 
+// The one-launch kernel of token_narrow.h: 16-bit types, up to 128 channels, nothing kept, and rows for half of the CUs at least
+// (a workgroup walks all hidden channels by itself).
+bool narrow_fits(const sr355_ffn_args *a) {
+    return !a->saved_dev && a->dtype != SR355_DTYPE_F32 && a->channels <= 128 && a->rows >= 64LL * N_CU;
+}
+
 // up to so many rows the kernels of token_rows.h: reading the weights bounds them
 constexpr int FEW_ROWS = 64;
 
 struct ForwardPlan : Plan {
     Operand x, wg, wu, wd;
     void *g, *u, *h;
+    Operand bg = {nullptr, 0}, bu = {nullptr, 0};
     Splits down;
     float *parts = nullptr;
 
@@ -301,8 +309,14 @@ struct ForwardPlan : Plan {
             unsigned char *s = (unsigned char *)a->saved_dev;
             g = s, u = s + hidden_bytes(a), h = s + 2 * hidden_bytes(a);
         } else {
-            g = u = nullptr, h = take(hidden_bytes(a));
+            g = u = nullptr, h = nullptr;
         }
+        if (narrow_fits(a)) {
+            if (a->b_gate_dev) bg = operand(a->b_gate_dev, 1, a->hidden, hidden_ld(a), a->dtype);
+            if (a->b_up_dev) bu = operand(a->b_up_dev, 1, a->hidden, hidden_ld(a), a->dtype);
+            return;
+        }
+        if (!h) h = take(hidden_bytes(a));
         if (a->rows > FEW_ROWS) {
             down = product_splits(a->rows, a->channels, a->hidden, 1, a->dtype);
             if (down.n > 1) parts = (float *)take((size_t)down.n * a->rows * a->channels * sizeof(float));
@@ -416,11 +430,41 @@ int ffn_forward_few(const sr355_ffn_args *a, const ForwardPlan &p, hipStream_t s
     return few_rows_both<T, 4>(g, d, stream);
 }
 
+template <typename T, int CP, int KIND>
+void narrow_launch_width(const TokNarrowArgs &n, hipStream_t stream) {
+    const dim3 grid((unsigned)tok_cdiv(n.rows, TokNarrow<CP>::ROWS));
+    if (n.bg || n.bu) hipLaunchKernelGGL((tok_narrow_kernel<T, CP, KIND, true>), grid, dim3(256), 0, stream, n);
+    else hipLaunchKernelGGL((tok_narrow_kernel<T, CP, KIND, false>), grid, dim3(256), 0, stream, n);
+}
+template <typename T, int KIND>
+void narrow_launch(const TokNarrowArgs &n, hipStream_t stream) {
+    if (n.C <= 64) narrow_launch_width<T, 64, KIND>(n, stream);
+    else narrow_launch_width<T, 128, KIND>(n, stream);
+}
+
+template <typename T>
+int ffn_forward_narrow(const sr355_ffn_args *a, const ForwardPlan &p, hipStream_t stream) {
+    TokNarrowArgs n = {};
+    n.x = (const unsigned char *)p.x.p, n.x_ld = p.x.ld * sizeof(T);
+    n.wg = (const unsigned char *)p.wg.p, n.wu = (const unsigned char *)p.wu.p, n.w_ld = p.wg.ld * sizeof(T);
+    n.wd = (const unsigned char *)p.wd.p, n.wd_ld = p.wd.ld * sizeof(T);
+    n.bg = (const unsigned char *)p.bg.p, n.bu = (const unsigned char *)p.bu.p, n.bd = a->b_down_dev;
+    n.y = a->y_dev, n.y_ld = a->channels, n.rows = a->rows, n.C = a->channels, n.F = a->hidden, n.act = a->activation;
+    if (a->activation == SR355_ACT_SILU) narrow_launch<T, SR355_ACT_SILU>(n, stream);
+    else if (a->activation == SR355_ACT_GELU) narrow_launch<T, SR355_ACT_GELU>(n, stream);
+    else if (a->activation == SR355_ACT_RELU) narrow_launch<T, SR355_ACT_RELU>(n, stream);
+    else narrow_launch<T, SR355_ACT_SIGMOID>(n, stream);
+    return check_hip(hipGetLastError(), "gated_ffn narrow launch");
+}
+
 template <typename T>
 int ffn_forward(const sr355_ffn_args *a, hipStream_t stream) {
     ForwardPlan p(a, (unsigned char *)a->workspace_dev);
     int rc = run_pads<T>(p, stream);
     if (rc != SR355_OK) return rc;
+    if constexpr (sizeof(T) == 2) {
+        if (narrow_fits(a)) return ffn_forward_narrow<T>(a, p, stream);
+    }
     if (a->rows <= FEW_ROWS) return ffn_forward_few<T>(a, p, stream);
     TokGemmArgs g = {};
     g.n_jobs = 1, g.sections = 1, g.act = a->activation, g.K = a->channels;

@@ -138,23 +138,27 @@ __device__ __forceinline__ void tok_read(tok_v4u &f, tok_v2u &lo, tok_v2u &hi, u
 }
 
 // The activation and its derivative.  T = float goes through the exact functions, the 16-bit types through the hardware's
-// exp2 and reciprocal (errors of a few 2^-23, far below their own rounding).
+// exp2 and reciprocal (errors of a few 2^-23, far below their own rounding) and, for the normal distribution's integral, the
+// polynomial of Abramowitz and Stegun 7.1.26: erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2) with t = 1 / (1 + p x), x >= 0, absolute
+// error at most 1.5e-7.  The library's erff takes some 45 instructions an element, which bounded the forward pass of
+// 262144 x 64 x 256 (130 us for the gate and up launch); this takes 15 and shares the exponential with the derivative.
 template <bool EXACT>
 __device__ __forceinline__ float tok_sigmoid(float g) {
     if constexpr (EXACT) return 1.0f / (1.0f + expf(-g));
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896f * g));
 }
+// the integral up to g and the density (without its 1 / sqrt(2 pi)) of the normal distribution
 template <bool EXACT>
-__device__ __forceinline__ float tok_gauss(float g) {      // exp(-g^2 / 2)
-    if constexpr (EXACT) return expf(-0.5f * g * g);
-    return __builtin_amdgcn_exp2f(-0.72134752044448f * g * g);
-}
-template <bool EXACT, int KIND>
-__device__ __forceinline__ float tok_act(float g) {
-    if constexpr (KIND == SR355_ACT_SILU) return g * tok_sigmoid<EXACT>(g);
-    if constexpr (KIND == SR355_ACT_GELU) return g * (0.5f * (1.0f + erff(0.70710678118655f * g)));
-    if constexpr (KIND == SR355_ACT_RELU) return g < 0.f ? 0.f : g;       // (a NaN stays one)
-    return tok_sigmoid<EXACT>(g);
+__device__ __forceinline__ void tok_normal(float g, float &cdf, float &density) {
+    if constexpr (EXACT) {
+        cdf = 0.5f * (1.0f + erff(0.70710678118655f * g)), density = expf(-0.5f * g * g);
+    } else {
+        density = __builtin_amdgcn_exp2f(-0.72134752044448f * g * g);
+        const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * 0.70710678118655f * fabsf(g));
+        const float poly = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+        const float tail = 0.5f * poly * density;
+        cdf = g < 0.f ? tail : 1.0f - tail;
+    }
 }
 template <bool EXACT, int KIND>
 __device__ __forceinline__ void tok_act_grad(float g, float &a, float &da) {
@@ -162,13 +166,20 @@ __device__ __forceinline__ void tok_act_grad(float g, float &a, float &da) {
         const float s = tok_sigmoid<EXACT>(g);
         a = g * s, da = s * (1.0f + g * (1.0f - s));
     } else if constexpr (KIND == SR355_ACT_GELU) {
-        const float cdf = 0.5f * (1.0f + erff(0.70710678118655f * g));
-        a = g * cdf, da = cdf + g * (0.39894228040143f * tok_gauss<EXACT>(g));
+        float cdf, density;
+        tok_normal<EXACT>(g, cdf, density);
+        a = g * cdf, da = cdf + g * (0.39894228040143f * density);
     } else if constexpr (KIND == SR355_ACT_RELU) {
-        a = g < 0.f ? 0.f : g, da = g > 0.f ? 1.0f : 0.f;
+        a = g < 0.f ? 0.f : g, da = g > 0.f ? 1.0f : 0.f;                 // (a NaN stays one)
     } else {
         a = tok_sigmoid<EXACT>(g), da = a * (1.0f - a);
     }
+}
+template <bool EXACT, int KIND>
+__device__ __forceinline__ float tok_act(float g) {
+    float a, da;
+    tok_act_grad<EXACT, KIND>(g, a, da);
+    return a;
 }
 
 // Eight consecutive elements, in 16-byte accesses.

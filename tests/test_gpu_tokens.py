@@ -288,6 +288,40 @@ def test_gated_ffn_is_exact_on_small_integers(shape, dtype):
         assert torch.equal(tokens.gated_ffn(x, *ws, *bs, activation="relu"), y)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(16384, 64, 256), (16500, 1, 1), (16400, 33, 70), (20001, 128, 96), (16384, 72, 520), (16391, 8, 1000),
+                                   (16640, 96, 31)])
+def test_gated_ffn_unrecorded_on_many_narrow_rows_is_exact_on_small_integers(shape, dtype):
+    """Forward only, up to 128 channels (16-bit types: one launch that keeps the hidden channels in registers)."""
+    t, c, f = shape
+    x = sparse_ints(t, c, 3, 11, dtype)
+    ws = [ternary(f, c, 12, dtype), ternary(f, c, 13, dtype), ternary(c, f, 14, dtype)]
+    bs = [ternary(1, n, 15 + i, dtype)[0] for i, n in enumerate((f, f, c))]
+    xd, wg, wu, wd, bg, bu, bd = (v.double() for v in (x, *ws, *bs))
+    for biases in (True, False):
+        g, u = xd @ wg.t().contiguous(), xd @ wu.t().contiguous()
+        if biases:
+            g, u = g + bg, u + bu
+        want = (g.clamp_min(0) * u) @ wd.t().contiguous() + (bd if biases else 0)
+        y = tokens.gated_ffn(x, *ws, *(bs if biases else ()), activation="relu")
+        assert torch.equal(y, want.to(dtype)), (biases, int((y != want.to(dtype)).sum()))
+    wide = torch.full((t, c + 5), float("nan"), dtype=dtype, device=DEV)       # rows of another stride, at an odd address
+    wide[:, 3:3 + c] = x
+    assert torch.equal(tokens.gated_ffn(wide[:, 3:3 + c], *ws, activation="relu"), y)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", list(ACTS))
+def test_gated_ffn_unrecorded_on_many_narrow_rows_matches_the_formula(act, dtype):
+    for c, f in ((64, 96), (100, 40)):
+        x, dy, ws, bs = ffn_inputs(16400, c, f, dtype, True, 35)
+        want, tol = ffn_bounds(x, dy, ws, bs, act, half_step(dtype))
+        within(tokens.gated_ffn(x, *ws, *bs, activation=act), want[0], tol[0] + torch.finfo(dtype).tiny * (1 + f), "y")
+        x[7, 3] = float("nan")
+        y = tokens.gated_ffn(x, *ws, *bs, activation=act)
+        assert y[7].isnan().all() and y[:7].isfinite().all() and y[8:].isfinite().all()
+
+
 def ffn_bounds(x, dy, ws, bs, act, u):
     """Results and bounds in 64 bits.  Per sum of n products: n B of the sum of magnitudes; u per rounding to the type."""
     t, c = x.shape
