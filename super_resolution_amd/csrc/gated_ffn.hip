@@ -37,28 +37,32 @@ struct PadJob {
 struct PadArgs {
     PadJob job[6];
 };
-// rows of `cols` elements into rows of dst_ld (a multiple of a unit), zeros behind
+// Rows of `cols` elements into rows of dst_ld (whole units), zeros behind.  Neither side of an odd row is aligned to more than
+// an element, so a wave moves 64 neighbouring elements an instruction, eight of them in flight.
 template <typename T>
 __global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs p) {
-    constexpr int E = 16 / sizeof(T);
+    constexpr int UN = 8;
     const PadJob &j = p.job[blockIdx.y];
-    const long long units = j.dst_ld / E, n = j.rows * units;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-        const long long row = i / units;
-        const int c = (int)(i - row * units) * E;
-        const T *src = (const T *)j.src + row * j.src_ld + c;
-        TokUnit<T> u;
+    const int lane = threadIdx.x & 63;
+    const long long per_row = (j.dst_ld + 64 * UN - 1) / (64 * UN), n = j.rows * per_row;
+    for (long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += (long long)gridDim.x * 4) {
+        const long long row = i / per_row;
+        const int c0 = (int)(i - row * per_row) * 64 * UN + lane;
+        const T *src = (const T *)j.src + row * j.src_ld;
+        T *dst = (T *)j.dst + row * j.dst_ld, v[UN];
 #pragma unroll
-        for (int e = 0; e < E; ++e) u.v[e] = c + e < j.cols ? src[e] : (T)0.f;
-        tok_store_unit((T *)j.dst + i * E, u);
+        for (int k = 0; k < UN; ++k) v[k] = c0 + k * 64 < j.cols ? src[c0 + k * 64] : (T)0.f;
+#pragma unroll
+        for (int k = 0; k < UN; ++k)
+            if (c0 + k * 64 < j.dst_ld) dst[c0 + k * 64] = v[k];
     }
 }
 
 // out[j] = sum over splits, in order, of part[s * n + j]
 struct ReduceArgs {
-    const float *part[3];
-    void *out[3];
-    long long n[3];
+    const float *part[6];
+    void *out[6];
+    long long n[6];
     int splits;
     const void *bias;        // of columns (job 0), may be null
     int cols;
@@ -96,52 +100,9 @@ __global__ __launch_bounds__(256) void reduce_splits_kernel(ReduceArgs a) {
     }
 }
 
-// Column sums of up to three matrices of rows (16-byte rows): workgroup (part, block of 32 units, matrix), thread
-// (unit, one of 8 row groups); the row groups meet in the LDS.
-struct ColJob {
-    const void *src;
-    long long ld, first;     // first: column of the job in a partial row
-    int cols;
-};
-struct ColArgs {
-    ColJob job[3];
-    float *parts;
-    long long rows, stride;
-};
-template <typename T>
-__global__ __launch_bounds__(256) void column_sums_kernel(ColArgs a) {
-    constexpr int E = 16 / sizeof(T);
-    __shared__ float red[8][32 * E + 1];
-    const ColJob &j = a.job[blockIdx.z];
-    const int ul = threadIdx.x & 31, rg = threadIdx.x >> 5;
-    const int c = (blockIdx.y * 32 + ul) * E;
-    float s[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) s[e] = 0.f;
-    if (c < j.cols) {
-        for (long long r = (long long)blockIdx.x * 8 + rg; r < a.rows; r += (long long)gridDim.x * 8) {
-            float v[E];
-            tok_load<T, E>((const T *)j.src + r * j.ld + c, v);
-#pragma unroll
-            for (int e = 0; e < E; ++e) s[e] += v[e];
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) red[rg][ul * E + e] = s[e];
-    __syncthreads();
-    for (int k = threadIdx.x; k < 32 * E; k += 256) {
-        const int col = blockIdx.y * 32 * E + k;
-        if (col >= j.cols) continue;
-        float t = 0.f;
-        for (int r = 0; r < 8; ++r) t += red[r][k];
-        a.parts[(size_t)blockIdx.x * a.stride + j.first + col] = t;
-    }
-}
-constexpr int COL_PARTS = 128;
-
-template <typename T, typename G, bool A_RC, bool B_RC, int EPI>
+template <typename T, typename G, bool A_RC, bool B_RC, int EPI, bool SUMS = false>
 int gemm_launch(const TokGemmArgs &g, const char *what, hipStream_t stream) {
-    void (*const kernel)(TokGemmArgs) = tok_gemm_kernel<T, G, A_RC, B_RC, EPI>;
+    void (*const kernel)(TokGemmArgs) = tok_gemm_kernel<T, G, A_RC, B_RC, EPI, SUMS>;
     if (G::LDS_BYTES > 64 * 1024) {
         // (per device, and cheap: not remembered)
         const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS_BYTES);
@@ -267,11 +228,11 @@ int run_pads(const Plan &plan, hipStream_t stream) {
     if (!plan.n_pads) return SR355_OK;
     long long most = 0;
     for (int i = 0; i < plan.n_pads; ++i) {
-        const long long n = plan.pads.job[i].rows * plan.pads.job[i].dst_ld * (long long)sizeof(T) / 16;
+        const long long n = plan.pads.job[i].rows * tok_cdiv(plan.pads.job[i].dst_ld, 512);
         if (n > most) most = n;
     }
     if (most == 0) return SR355_OK;
-    const long long wgs = tok_cdiv(most, 256);
+    const long long wgs = tok_cdiv(most, 4);
     hipLaunchKernelGGL((pad_rows_kernel<T>), dim3((unsigned)(wgs > 4096 ? 4096 : wgs), plan.n_pads), dim3(256), 0, stream, plan.pads);
     return check_hip(hipGetLastError(), "gated_ffn row padding launch");
 }
@@ -326,16 +287,17 @@ struct ForwardPlan : Plan {
     bool split = false;
 };
 
-// The weight gradients: k is the rows.
+// The weight gradients, and with them the bias gradients as their left operands' sums: k is the rows.  A bias whose weight
+// needs no gradient takes a product with one column that is not stored.
 struct WgradShape {
     bool big;
     Splits split;
 };
 template <typename G>
 long long wgrad_tiles(const sr355_ffn_args *a) {
-    const long long f_c = tok_cdiv(a->hidden, G::BM) * tok_cdiv(a->channels, G::BN);
-    const long long c_f = tok_cdiv(a->channels, G::BM) * tok_cdiv(a->hidden, G::BN);
-    return (a->dw_gate_dev ? f_c : 0) + (a->dw_up_dev ? f_c : 0) + (a->dw_down_dev ? c_f : 0);
+    auto tiles = [](int M, int N, const void *w, const void *b) { return w || b ? tok_cdiv(M, G::BM) * tok_cdiv(w ? N : 1, G::BN) : 0; };
+    return tiles(a->hidden, a->channels, a->dw_gate_dev, a->db_gate_dev) + tiles(a->hidden, a->channels, a->dw_up_dev, a->db_up_dev) +
+           tiles(a->channels, a->hidden, a->dw_down_dev, a->db_down_dev);
 }
 template <typename G>
 Splits wgrad_splits(const sr355_ffn_args *a, int slots) {
@@ -352,15 +314,15 @@ struct BackwardPlan : Plan {
     Operand x, dy, wg, wu, wd;
     void *dg, *du;
     const void *g, *u, *h;
-    float *parts, *col_parts, *dx_parts;
+    float *parts, *row_parts, *dx_parts;
     WgradShape wgrad;
     Splits dx;
     bool need_hidden;
 
     BackwardPlan(const sr355_ffn_args *a, unsigned char *ws) {
         base = ws;
-        const bool gate_up = a->dw_gate_dev || a->dw_up_dev;
-        need_hidden = a->dx_dev || gate_up || a->db_gate_dev || a->db_up_dev;
+        const bool gate_up = a->dw_gate_dev || a->dw_up_dev || a->db_gate_dev || a->db_up_dev;
+        need_hidden = a->dx_dev || gate_up;
         x = wg = wu = wd = {nullptr, 0};
         dy = operand(a->dy_dev, a->rows, a->channels, a->dy_ld, a->dtype);
         if (gate_up) x = operand(a->x_dev, a->rows, a->channels, a->x_ld, a->dtype);
@@ -380,8 +342,7 @@ struct BackwardPlan : Plan {
         dx = {1, 0};
         if (a->dx_dev && a->rows > 0) dx = product_splits(a->rows, a->channels, a->hidden, 2, a->dtype);
         dx_parts = dx.n > 1 ? (float *)take((size_t)dx.n * a->rows * a->channels * sizeof(float)) : nullptr;
-        const bool cols = a->db_gate_dev || a->db_up_dev || a->db_down_dev;
-        col_parts = cols ? (float *)take((size_t)COL_PARTS * (2 * hidden_ld(a) + dy.ld) * sizeof(float)) : nullptr;
+        row_parts = wgrad.split.n > 1 ? (float *)take((size_t)wgrad.split.n * (2 * (size_t)a->hidden + a->channels) * sizeof(float)) : nullptr;
     }
 };
 
@@ -484,41 +445,48 @@ int ffn_forward(const sr355_ffn_args *a, hipStream_t stream) {
     return product_launch<T, false>(d, p.down, p.split ? p.parts : nullptr, "gated_ffn down launch", stream);
 }
 
+template <typename T, typename G, bool SUMS>
+int wgrad_launch(TokGemmArgs &g, bool part, hipStream_t stream) {
+    set_tiles<G>(g, false);
+    return part ? gemm_launch<T, G, true, true, TOK_EPI_PART, SUMS>(g, "gated_ffn weight gradient launch", stream)
+                : gemm_launch<T, G, true, true, TOK_EPI_STORE, SUMS>(g, "gated_ffn weight gradient launch", stream);
+}
+
 template <typename T>
 int ffn_wgrad(const sr355_ffn_args *a, const BackwardPlan &p, hipStream_t stream) {
     TokGemmArgs g = {};
     g.sections = 1, g.K = (int)a->rows, g.splits = p.wgrad.split.n, g.split_stages = p.wgrad.split.stages;
     ReduceArgs r = {};
-    float *parts = p.parts;
+    float *parts = p.parts, *row_parts = p.row_parts;
     const size_t n = (size_t)a->hidden * a->channels;
-    auto add = [&](const void *l, long long l_ld, const void *q, long long q_ld, int M, int N, void *out) {
-        if (!out) return;
-        TokJob &j = g.job[g.n_jobs];
+    int n_out = 0;
+    auto add = [&](const void *l, long long l_ld, const void *q, long long q_ld, int M, int N, void *out, void *sums) {
+        if (!out && !sums) return;
+        TokJob &j = g.job[g.n_jobs++];
         j.a[0] = (const unsigned char *)l, j.a_ld = l_ld * sizeof(T);
         j.b[0] = (const unsigned char *)q, j.b_ld = q_ld * sizeof(T);
-        j.M = M, j.N = N, j.c = out, j.c_ld = N, j.part = parts;
-        r.part[g.n_jobs] = parts, r.out[g.n_jobs] = out, r.n[g.n_jobs] = (long long)n;
-        if (parts) parts += p.wgrad.split.n * n;
-        ++g.n_jobs;
+        j.M = M, j.N = out ? N : 1, j.c = out, j.c_ld = N, j.row_sums = sums;
+        if (g.splits == 1) return;
+        if (out) {
+            j.part = parts, parts += g.splits * n;
+            r.part[n_out] = j.part, r.out[n_out] = out, r.n[n_out++] = (long long)n;
+        }
+        if (sums) {
+            j.row_part = row_parts, row_parts += (size_t)g.splits * M;
+            r.part[n_out] = j.row_part, r.out[n_out] = sums, r.n[n_out++] = M;
+        }
     };
-    add(p.dg, hidden_ld(a), p.x.p, p.x.ld, a->hidden, a->channels, a->dw_gate_dev);
-    add(p.du, hidden_ld(a), p.x.p, p.x.ld, a->hidden, a->channels, a->dw_up_dev);
-    add(p.dy.p, p.dy.ld, p.h, hidden_ld(a), a->channels, a->hidden, a->dw_down_dev);
+    add(p.dg, hidden_ld(a), p.x.p, p.x.ld, a->hidden, a->channels, a->dw_gate_dev, a->db_gate_dev);
+    add(p.du, hidden_ld(a), p.x.p, p.x.ld, a->hidden, a->channels, a->dw_up_dev, a->db_up_dev);
+    add(p.dy.p, p.dy.ld, p.h, hidden_ld(a), a->channels, a->hidden, a->dw_down_dev, a->db_down_dev);
     if (!g.n_jobs) return SR355_OK;
-    const char *what = "gated_ffn weight gradient launch";
-    int rc;
-    if (p.wgrad.big) {
-        set_tiles<TileWgrad>(g, false);
-        rc = p.parts ? gemm_launch<T, TileWgrad, true, true, TOK_EPI_PART>(g, what, stream)
-                     : gemm_launch<T, TileWgrad, true, true, TOK_EPI_STORE>(g, what, stream);
-    } else {
-        set_tiles<Tile128>(g, false);
-        rc = p.parts ? gemm_launch<T, Tile128, true, true, TOK_EPI_PART>(g, what, stream)
-                     : gemm_launch<T, Tile128, true, true, TOK_EPI_STORE>(g, what, stream);
-    }
-    if (rc != SR355_OK || !p.parts) return rc;
+    const bool part = g.splits > 1;
+    const bool sums = a->db_gate_dev || a->db_up_dev || a->db_down_dev;
+    const int rc = p.wgrad.big ? (sums ? wgrad_launch<T, TileWgrad, true>(g, part, stream) : wgrad_launch<T, TileWgrad, false>(g, part, stream))
+                               : (sums ? wgrad_launch<T, Tile128, true>(g, part, stream) : wgrad_launch<T, Tile128, false>(g, part, stream));
+    if (rc != SR355_OK || !part) return rc;
     r.splits = p.wgrad.split.n;
-    return reduce_launch<T>(r, g.n_jobs, "gated_ffn weight gradient reduction launch", stream);
+    return reduce_launch<T>(r, n_out, "gated_ffn weight gradient reduction launch", stream);
 }
 
 template <typename T>
@@ -547,30 +515,7 @@ int ffn_backward(const sr355_ffn_args *a, hipStream_t stream) {
         rc = product_launch<T, true>(g, p.dx, p.dx_parts, "gated_ffn data gradient launch", stream);
         if (rc != SR355_OK) return rc;
     }
-    rc = ffn_wgrad<T>(a, p, stream);
-    if (rc != SR355_OK || !p.col_parts) return rc;
-    constexpr int E = 16 / sizeof(T);
-    ColArgs c = {};
-    c.parts = p.col_parts, c.rows = a->rows, c.stride = 2 * hidden_ld(a) + p.dy.ld;
-    int n = 0, most = 0;
-    auto add = [&](const void *src, long long ld, long long first, int cols, const void *wanted) {
-        if (!wanted) return;
-        c.job[n++] = {src, ld, first, cols};
-        if (cols > most) most = cols;
-    };
-    add(p.dg, hidden_ld(a), 0, a->hidden, a->db_gate_dev);
-    add(p.du, hidden_ld(a), hidden_ld(a), a->hidden, a->db_up_dev);
-    add(p.dy.p, p.dy.ld, 2 * hidden_ld(a), a->channels, a->db_down_dev);
-    const int n_parts = (int)(tok_cdiv(a->rows, 8) < COL_PARTS ? tok_cdiv(a->rows, 8) : COL_PARTS);
-    if (n_parts > 0) {
-        hipLaunchKernelGGL((column_sums_kernel<T>), dim3(n_parts, (unsigned)tok_cdiv(most, 32 * E), n), dim3(256), 0, stream, c);
-        rc = check_hip(hipGetLastError(), "gated_ffn bias gradient launch");
-        if (rc != SR355_OK) return rc;
-    }
-    const long long first[3] = {0, hidden_ld(a), 2 * hidden_ld(a)};
-    const int count[3] = {a->hidden, a->hidden, a->channels};
-    void *const out[3] = {a->db_gate_dev, a->db_up_dev, a->db_down_dev};
-    return launch_tok_sum_parts(p.col_parts, n_parts, c.stride, first, count, out, 3, a->dtype, stream);
+    return ffn_wgrad<T>(a, p, stream);
 }
 }  // namespace
 

@@ -37,6 +37,8 @@ struct TokJob {
     long long c_ld;                     // elements
     const void *bias;                   // [N] of T, may be null
     float *part;                        // split products: [splits][M][N] fp32 partials
+    void *row_sums;                     // A strided in k: [M] of T, sums of A over k (may be null; c may be null with it)
+    float *row_part;                    // split products: [splits][M] fp32 partials of them
     int tiles_m, tiles_n;
 };
 struct TokGemmArgs {
@@ -196,7 +198,7 @@ __device__ __forceinline__ void tok_load8(const T *p, float (&v)[8]) {
     for (int j = 0; j < 8; j += E) tok_load<T, E>(p + j, *reinterpret_cast<float(*)[E]>(v + j));
 }
 
-template <typename T, typename G, bool A_RC, bool B_RC, int EPI>
+template <typename T, typename G, bool A_RC, bool B_RC, int EPI, bool SUMS>
 __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
     typedef TokImage<T, G::BM, G::KB, A_RC> IA;
     typedef TokImage<T, G::BN, G::KB, B_RC> IB;
@@ -344,6 +346,25 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
     // fragments of two k steps: the one being multiplied and the next
+    // Sums of A over k (the bias gradients, for which A would be read again): the waves of the first column of tiles that hold
+    // its first columns add up the fragments as they pass, one lane per row and half of k.  A variant of its own: the branch
+    // in the main loop costs 7 % where nothing is summed.
+    static_assert(!SUMS || (A_RC && (EPI == TOK_EPI_STORE || EPI == TOK_EPI_PART)), "sums of a left operand strided in k");
+    const bool sums = SUMS && tn == 0 && wn == 0 && job.row_sums;
+    float row_sum[SUMS ? MT : 1];
+#pragma unroll
+    for (int i = 0; i < (SUMS ? MT : 1); ++i) row_sum[i] = 0.f;
+    auto add_sums = [&](const tok_v4u (&a)[MT]) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            T v[E];
+            __builtin_memcpy(v, &a[i], 16);
+            float s = (float)v[0];
+#pragma unroll
+            for (int e = 1; e < E; ++e) s += (float)v[e];
+            row_sum[i] += s;
+        }
+    };
     struct Frags {
         tok_v4u a[MT], b[NT];
         tok_v2u alo[MT], ahi[MT], blo[NT], bhi[NT];
@@ -434,6 +455,9 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
                 __builtin_amdgcn_s_barrier();
                 asm volatile("" ::: "memory");
             }
+            if constexpr (SUMS) {
+                if (sums) add_sums(f.a);
+            }
             __builtin_amdgcn_sched_barrier(0);
             constexpr int SHARE0 = LAST ? 0 : FIRST_PART, SHARE1 = LAST ? FIRST_PART : (S == 0 ? CA + CB : FIRST_PART);
             tok_static_for<MFMAS>([&](auto mm) {
@@ -474,6 +498,20 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
     // and its fetch took longer than the main loop (training step of 16384 x 1024 x 4096: 354 + 310 us for the two products
     // with an activation).
     constexpr bool EXACT = sizeof(T) == 4;
+    if constexpr (SUMS) {
+        if (sums) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const float s = row_sum[i] + __shfl_xor(row_sum[i], 32, 64);
+                const long long m = m0 + (wm * MT + i) * 32 + (lane & 31);
+                if (lane < 32 && m < job.M) {
+                    if constexpr (EPI == TOK_EPI_PART) job.row_part[(size_t)split * job.M + m] = s;
+                    else ((T *)job.row_sums)[m] = (T)s;
+                }
+            }
+        }
+        if (!(EPI == TOK_EPI_PART ? (const void *)job.part : job.c)) return;
+    }
     constexpr int CHUNKS = NT * 8;                          // of 4 columns
     constexpr int COLS = EPI == TOK_EPI_GLU ? NT * 16 : NT * 32;
     constexpr int LANES = COLS / 8, ROWS = 64 / LANES;      // lanes of a row, rows of an instruction
@@ -584,9 +622,9 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
     }
 }
 
-template <typename T, typename G, bool A_RC, bool B_RC, int EPI>
+template <typename T, typename G, bool A_RC, bool B_RC, int EPI, bool SUMS = false>
 __global__ __launch_bounds__(G::THREADS) void tok_gemm_kernel(TokGemmArgs p) {
-    tok_gemm_body<T, G, A_RC, B_RC, EPI>(p);
+    tok_gemm_body<T, G, A_RC, B_RC, EPI, SUMS>(p);
 }
 
 }  // namespace
