@@ -6,10 +6,8 @@
 // the gate and the up weights of the same hidden channels, so g and u meet in a wave's registers), one the projection back.
 // Training keeps act(g), u act'(g) and h, inference h alone.  Backward: one launch computes dh and, in its epilogue, dg and
 // du (two products per element: the derivative is taken in the forward pass, from g and u as they were accumulated); one dx,
-// over both sections of k; one all three weight gradients.  Products accumulate in fp32.  Between the launches the hidden
-// channels are held in the type of x: h, dg and du are rounded to it as operands of products in any case, and the two kept
-// factors in fp32 would double the traffic of the two launches that are nearest to the memory's pace (134 MB per array for
-// 16384 rows of 4096).
+// over both sections of k; one all three weight gradients and the bias gradients.  Products accumulate in fp32.  Between the
+// launches h, dg and du are held in the type of x, to which they are rounded as operands of products in any case.
 //
 // Operands are read 16 bytes at a time.  What does not allow that (a width, stride or pointer that is no multiple of 16
 // bytes) is first copied into padded rows of the workspace, one launch for all of them.
@@ -253,9 +251,27 @@ bool narrow_fits(const sr355_ffn_args *a) {
 // up to so many rows the kernels of token_rows.h: reading the weights bounds them
 constexpr int FEW_ROWS = 64;
 
+// a call's saved buffer: h, the two kept arrays, their low parts
+struct Saved {
+    TokKept kept = {};
+    void *h = nullptr;
+    size_t bytes = 0;
+    Saved(const sr355_ffn_args *a, unsigned char *base) {
+        auto take = [&](size_t n) {
+            void *r = base ? base + bytes : nullptr;
+            bytes += (n + 255) & ~(size_t)255;
+            return r;
+        };
+        h = take(hidden_bytes(a)), kept.a = take(hidden_bytes(a)), kept.d = take(hidden_bytes(a));
+        if (a->dtype == SR355_DTYPE_F32) return;
+        kept.a_low = (unsigned char *)take((size_t)a->rows * hidden_ld(a)), kept.d_low = (unsigned char *)take((size_t)a->rows * hidden_ld(a));
+    }
+};
+
 struct ForwardPlan : Plan {
     Operand x, wg, wu, wd;
-    void *g, *u, *h;
+    TokKept kept = {};
+    void *h = nullptr;
     Operand bg = {nullptr, 0}, bu = {nullptr, 0};
     Splits down;
     float *parts = nullptr;
@@ -267,10 +283,8 @@ struct ForwardPlan : Plan {
         wu = operand(a->w_up_dev, a->hidden, a->channels, a->channels, a->dtype);
         wd = operand(a->w_down_dev, a->channels, a->hidden, a->hidden, a->dtype);
         if (a->saved_dev) {
-            unsigned char *s = (unsigned char *)a->saved_dev;
-            g = s, u = s + hidden_bytes(a), h = s + 2 * hidden_bytes(a);
-        } else {
-            g = u = nullptr, h = nullptr;
+            const Saved s(a, (unsigned char *)a->saved_dev);
+            kept = s.kept, h = s.h;
         }
         if (narrow_fits(a)) {
             if (a->b_gate_dev) bg = operand(a->b_gate_dev, 1, a->hidden, hidden_ld(a), a->dtype);
@@ -313,7 +327,8 @@ WgradShape wgrad_shape(const sr355_ffn_args *a) {
 struct BackwardPlan : Plan {
     Operand x, dy, wg, wu, wd;
     void *dg, *du;
-    const void *g, *u, *h;
+    TokKept kept;
+    const void *h;
     float *parts, *row_parts, *dx_parts;
     WgradShape wgrad;
     Splits dx;
@@ -331,8 +346,8 @@ struct BackwardPlan : Plan {
             wu = operand(a->w_up_dev, a->hidden, a->channels, a->channels, a->dtype);
         }
         if (need_hidden) wd = operand(a->w_down_dev, a->channels, a->hidden, a->hidden, a->dtype);
-        const unsigned char *s = (const unsigned char *)a->saved_dev;
-        g = s, u = s + hidden_bytes(a), h = s + 2 * hidden_bytes(a);
+        const Saved s(a, (unsigned char *)a->saved_dev);
+        kept = s.kept, h = s.h;
         dg = need_hidden ? take(hidden_bytes(a)) : nullptr;
         du = need_hidden ? take(hidden_bytes(a)) : nullptr;
         wgrad = wgrad_shape(a);
@@ -380,7 +395,7 @@ int ffn_forward_few(const sr355_ffn_args *a, const ForwardPlan &p, hipStream_t s
     g.w = (const unsigned char *)p.wg.p, g.w2 = (const unsigned char *)p.wu.p, g.w_ld = p.wg.ld * sizeof(T);
     g.rows = (int)a->rows, g.N = a->hidden, g.k_bytes = (int)(a->channels * sizeof(T));
     g.bias = a->b_gate_dev, g.bias2 = a->b_up_dev, g.act = a->activation;
-    g.out = p.h, g.kept_a = p.g, g.kept_d = p.u, g.out_ld = hidden_ld(a), g.n_store = (int)hidden_ld(a);
+    g.out = p.h, g.kept = p.kept, g.out_ld = hidden_ld(a), g.n_store = (int)hidden_ld(a);
     TokRowsArgs d = {};
     d.x = (const unsigned char *)p.h, d.x_ld = hidden_ld(a) * sizeof(T);
     d.w = (const unsigned char *)p.wd.p, d.w_ld = p.wd.ld * sizeof(T);
@@ -433,7 +448,7 @@ int ffn_forward(const sr355_ffn_args *a, hipStream_t stream) {
     j.a[0] = (const unsigned char *)p.x.p, j.a_ld = p.x.ld * sizeof(T);
     j.b[0] = (const unsigned char *)p.wg.p, j.b[1] = (const unsigned char *)p.wu.p, j.b_ld = p.wg.ld * sizeof(T);
     j.M = (int)a->rows, j.N = a->hidden, j.bias = a->b_gate_dev;
-    g.bias_up = a->b_up_dev, g.g = p.g, g.u = p.u, g.h = p.h, g.h_ld = hidden_ld(a);
+    g.bias_up = a->b_up_dev, g.kept = p.kept, g.h = p.h, g.h_ld = hidden_ld(a);
     rc = gemm_pick<T, false, false, TOK_EPI_GLU>(g, "gated_ffn gate / up launch", stream);
     if (rc != SR355_OK) return rc;
     TokGemmArgs d = {};
@@ -501,7 +516,7 @@ int ffn_backward(const sr355_ffn_args *a, hipStream_t stream) {
         j.a[0] = (const unsigned char *)p.dy.p, j.a_ld = p.dy.ld * sizeof(T);
         j.b[0] = (const unsigned char *)p.wd.p, j.b_ld = p.wd.ld * sizeof(T);
         j.M = (int)a->rows, j.N = a->hidden;
-        g.g = p.dg, g.u = p.du, g.sg = p.g, g.su = p.u, g.h_ld = hidden_ld(a);
+        g.g = p.dg, g.u = p.du, g.kept = p.kept, g.h_ld = hidden_ld(a);
         rc = gemm_pick<T, false, true, TOK_EPI_GLU_GRAD>(g, "gated_ffn hidden gradient launch", stream);
         if (rc != SR355_OK) return rc;
     }
@@ -527,7 +542,7 @@ extern "C" {
 
 size_t sr355_gated_ffn_saved_bytes(const sr355_ffn_args *a) {
     if (!ffn_args_ok("gated_ffn_saved_bytes", a, false)) return 0;
-    return 3 * hidden_bytes(a) + 256;
+    return Saved(a, nullptr).bytes + 256;
 }
 
 size_t sr355_gated_ffn_workspace_bytes(const sr355_ffn_args *a, int backward) {

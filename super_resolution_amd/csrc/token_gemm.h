@@ -28,6 +28,24 @@ typedef _Float16 tok_f16x8 __attribute__((ext_vector_type(8)));
 typedef float tok_f32x4 __attribute__((ext_vector_type(4)));
 typedef float tok_f32x16 __attribute__((ext_vector_type(16)));
 
+// What the backward pass reads: act(g) and u act'(g).  fp32 is kept whole; for the 16-bit types the upper 24 bits of the
+// fp32 values are kept, 16 and 8 apart.  Kept in 16 bits they put a third rounding into every gradient behind the hidden
+// channels, beside those of dg / du and of the result (bf16: relative error 2.9e-3, now 2.4e-3; one rounding is 1.7e-3).
+struct TokKept {
+    void *a, *d;                        // [rows][h_ld] of 2 (4) bytes
+    unsigned char *a_low, *d_low;       // [rows][h_ld], null for fp32
+};
+template <typename T>
+__device__ __forceinline__ void tok_keep(void *at16, unsigned char *at8, long long at, float v) {
+    if constexpr (sizeof(T) == 4) {
+        ((float *)at16)[at] = v;
+    } else {
+        const unsigned b = __builtin_bit_cast(unsigned, v);
+        ((unsigned short *)at16)[at] = (unsigned short)(b >> 16);
+        at8[at] = (unsigned char)(b >> 8);
+    }
+}
+
 // One product of a launch.
 struct TokJob {
     const unsigned char *a[2], *b[2];   // operands of the (up to two) sections of k; GLU: b = gate and up weights
@@ -49,8 +67,8 @@ struct TokGemmArgs {
     int splits, split_stages;           // stages of one split
     int act;
     const void *bias_up;                // GLU
-    void *g, *u, *h;                    // GLU: act(g), u act'(g) (both or none) and the product; gradient: dg, du (in g, u)
-    const void *sg, *su;                // gradient: act(g), u act'(g)
+    TokKept kept;                       // GLU: written where not null; gradient: read
+    void *g, *u, *h;                    // GLU: the product (h); gradient: dg, du
     long long h_ld;                     // elements, of g / u / h / dg / du; a multiple of 16 bytes
 };
 
@@ -184,6 +202,47 @@ __device__ __forceinline__ float tok_act(float g) {
     return a;
 }
 
+// Eight kept values at a multiple of eight.
+template <typename T>
+__device__ __forceinline__ void tok_keep8(void *at16, unsigned char *at8, long long at, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) tok_store<float, 4>((float *)at16 + at + j, *reinterpret_cast<const float(*)[4]>(v + j));
+    } else {
+        tok_v4u high;
+        tok_v2u low;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const unsigned b0 = __builtin_bit_cast(unsigned, v[2 * j]), b1 = __builtin_bit_cast(unsigned, v[2 * j + 1]);
+            high[j] = (b0 >> 16) | (b1 & 0xffff0000u);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            unsigned w = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w |= (__builtin_bit_cast(unsigned, v[4 * j + k]) >> 8 & 0xffu) << (8 * k);
+            low[j] = w;
+        }
+        *reinterpret_cast<tok_v4u *>((unsigned short *)at16 + at) = high;
+        *reinterpret_cast<tok_v2u *>(at8 + at) = low;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void tok_kept8(const void *at16, const unsigned char *at8, long long at, float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) tok_load<float, 4>((const float *)at16 + at + j, *reinterpret_cast<float(*)[4]>(v + j));
+    } else {
+        const tok_v4u high = *reinterpret_cast<const tok_v4u *>((const unsigned short *)at16 + at);
+        const tok_v2u low = *reinterpret_cast<const tok_v2u *>(at8 + at);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const unsigned h = j & 1 ? high[j / 2] & 0xffff0000u : high[j / 2] << 16;
+            v[j] = __builtin_bit_cast(float, h | (low[j / 4] >> (8 * (j & 3)) & 0xffu) << 8);
+        }
+    }
+}
+
 // Eight consecutive elements, in 16-byte accesses.
 template <typename T>
 __device__ __forceinline__ void tok_store8(T *p, const float (&v)[8]) {
@@ -191,13 +250,6 @@ __device__ __forceinline__ void tok_store8(T *p, const float (&v)[8]) {
 #pragma unroll
     for (int j = 0; j < 8; j += E) tok_store<T, E>(p + j, *reinterpret_cast<const float(*)[E]>(v + j));
 }
-template <typename T>
-__device__ __forceinline__ void tok_load8(const T *p, float (&v)[8]) {
-    constexpr int E = 16 / sizeof(T);
-#pragma unroll
-    for (int j = 0; j < 8; j += E) tok_load<T, E>(p + j, *reinterpret_cast<float(*)[E]>(v + j));
-}
-
 template <typename T, typename G, bool A_RC, bool B_RC, int EPI, bool SUMS>
 __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
     typedef TokImage<T, G::BM, G::KB, A_RC> IA;
@@ -545,7 +597,7 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
                 const tok_f32x4 lo2 = turned(r, NT * 4 + col / 4), hi2 = turned(r, NT * 4 + col / 4 + 1);
                 float w[8] = {lo2[0], lo2[1], lo2[2], lo2[3], hi2[0], hi2[1], hi2[2], hi2[3]}, h[8];
                 const long long at = m * p.h_ld + n;
-                if (p.g) {
+                if (p.kept.a) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const float up = w[j] + bias2[j];
@@ -553,8 +605,8 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
                         tok_act_grad<EXACT, KIND>(v[j] + bias[j], v[j], da);
                         h[j] = v[j] * up, w[j] = up * da;
                     }
-                    tok_store8<T>((T *)p.g + at, v);
-                    tok_store8<T>((T *)p.u + at, w);
+                    tok_keep8<T>(p.kept.a, p.kept.a_low, at, v);
+                    tok_keep8<T>(p.kept.d, p.kept.d_low, at, w);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) h[j] = tok_act<EXACT, KIND>(v[j] + bias[j]) * (w[j] + bias2[j]);
@@ -563,8 +615,8 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
             } else if constexpr (EPI == TOK_EPI_GLU_GRAD) {
                 const long long at = m * p.h_ld + n;
                 float a[8], d[8];
-                tok_load8<T>((const T *)p.sg + at, a);
-                tok_load8<T>((const T *)p.su + at, d);
+                tok_kept8<T>(p.kept.a, p.kept.a_low, at, a);
+                tok_kept8<T>(p.kept.d, p.kept.d_low, at, d);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) d[j] *= v[j], a[j] *= v[j];
                 tok_store8<T>((T *)p.g + at, d);

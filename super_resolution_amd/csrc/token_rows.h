@@ -19,7 +19,8 @@ struct TokRowsArgs {
     int rows, N, k_bytes;
     int channels;                         // output channels of a workgroup: 16, or fewer where that leaves CUs idle
     const void *bias, *bias2;
-    void *out, *kept_a, *kept_d;          // GLU: h, act(g), u act'(g) (the last two may be null)
+    void *out;                            // GLU: h
+    TokKept kept;                         // GLU: written where not null
     long long out_ld;                     // elements
     int n_store;                          // columns stored (GLU: up to the padded row)
     int act;
@@ -122,9 +123,9 @@ __device__ __forceinline__ void tok_rows_body(const TokRowsArgs &p) {
             else if (p.act == SR355_ACT_RELU) tok_act_grad<EXACT, SR355_ACT_RELU>(v[0], a, d);
             else tok_act_grad<EXACT, SR355_ACT_SIGMOID>(v[0], a, d);
             ((T *)p.out)[at] = (T)(a * v[Q - 1]);
-            if (p.kept_a) {
-                ((T *)p.kept_a)[at] = (T)a;
-                ((T *)p.kept_d)[at] = (T)(v[Q - 1] * d);
+            if (p.kept.a) {
+                tok_keep<T>(p.kept.a, p.kept.a_low, at, a);
+                tok_keep<T>(p.kept.d, p.kept.d_low, at, v[Q - 1] * d);
             }
         } else {
             ((T *)p.out)[at] = (T)v[0];

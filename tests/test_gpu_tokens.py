@@ -345,14 +345,15 @@ def ffn_bounds(x, dy, ws, bs, act, u):
     e_h = e_a * uu.abs() + a.abs() * e_u + 2 * u * h.abs()
     y = h @ T(wd) + bd
     t_y = e_h @ T(wd.abs()) + (f + 4) * B * (h.abs() @ T(wd.abs()) + bd.abs()) + u * y.abs()
-    # the backward pass multiplies dh with act(g) and u act'(g), which are held rounded to the type: |a~ - a| <= e_a + u |a|
-    # and, with d = u act'(g), |d~ - d| <= (e_u |act'| + |u| e_act') (1 + ..) + u |d|
+    # the backward pass multiplies dh with act(g) and u act'(g), kept as the upper 24 bits of fp32 (cut: off by less than
+    # 2^-15): |a~ - a| <= e_a + 2^-15 |a| and, with d = u act'(g), |d~ - d| <= (e_u |act'| + |u| e_act') (1 + ..) + 2^-15 |d|
+    cut = 0.0 if u < 2.0 ** -20 else 2.0 ** -15
     e_dh = (c + 4) * B * (dyd.abs() @ wd.abs())
     e_da = 0.8 * e_g + fn * (1 + da.abs())
     if act == "relu":
         e_da = (g.abs() <= 2 * e_g).double()
-    e_as = e_a + 1.01 * u * a.abs()
-    e_d = e_u * (da.abs() + e_da) + uu.abs() * e_da + 1.01 * u * (uu * da).abs()
+    e_as = e_a + 1.01 * cut * a.abs()
+    e_d = e_u * (da.abs() + e_da) + uu.abs() * e_da + 1.01 * cut * (uu * da).abs() + 4 * B * (uu * da).abs()
     grow = 1.01
     e_dg = grow * (e_dh * (uu * da).abs() + dh.abs() * e_d + 4 * B * dg.abs()) + 1.01 * u * dg.abs()
     e_du = grow * (e_dh * a.abs() + dh.abs() * e_as + 4 * B * du.abs()) + 1.01 * u * du.abs()

@@ -37,7 +37,7 @@ def test_fakes_predict_shapes_and_types(dtype):
         wg, wd = torch.empty(40, 24, dtype=dtype, device="cuda"), torch.empty(24, 40, dtype=dtype, device="cuda")
         y, saved = torch.ops.sr355.gated_ffn_fwd(x, wg, wg, wd, None, None, None, 0, True)
         assert y.shape == x.shape and saved.dtype == torch.uint8
-        assert saved.numel() >= 3 * 15 * 40 * x.element_size()
+        assert saved.numel() >= 15 * 40 * (8 if dtype != torch.float32 else 12)
         g = torch.ops.sr355.gated_ffn_bwd(y, x, wg, wg, wd, saved, 0, [True] * 7)
         assert [tuple(t.shape) for t in g] == [(3, 5, 24), (40, 24), (40, 24), (24, 40), (40,), (40,), (24,)]
 
