@@ -364,7 +364,7 @@ int sr355_layer_norm_bwd(const void *dy_dev, long long dy_ld, const void *x_dev,
                          void *dx_dev, void *dw_dev, void *db_dev, void *workspace_dev, size_t workspace_bytes,
                          void *stream);
 
-/* y = (keep ? x / (1 - p) : 0) + skip over n contiguous elements (skip may be null); the gradient of x is the same call
+/* y = (keep ? x / (1 - p) : 0) + skip over n >= 1 contiguous elements (skip may be null); the gradient of x is the same call
  * on the gradient of y, without a skip.  Element i is kept by 16 bits of Philox 4x32 with 7 rounds, key rng[0], counter
  * (i / 8, rng[1] mod 2^32, site); p counts in steps of 2^-16.  rng: two 64-bit words in device memory. */
 int sr355_dropout(const void *x_dev, const void *skip_dev, long long n, int dtype, double p, const long long *rng_dev,

@@ -96,11 +96,10 @@ extern "C" {
 
 int sr355_dropout(const void *x, const void *skip, long long n, int dtype, double p, const long long *rng, unsigned site,
                   void *y, void *stream) {
-    if (n < 0 || !tok_dtype_ok(dtype) || !(p >= 0.0 && p <= 1.0)) {
-        set_error("dropout: bad arguments (n=%lld dtype=%d p=%g, p in [0, 1])", n, dtype, p);
+    if (n < 1 || !tok_dtype_ok(dtype) || !(p >= 0.0 && p <= 1.0)) {
+        set_error("dropout: bad arguments (n=%lld dtype=%d p=%g; at least one element, p in [0, 1])", n, dtype, p);
         return SR355_ERR_INVALID;
     }
-    if (n == 0) return SR355_OK;
     if (!x || !y || !rng) {
         set_error("dropout: null tensor");
         return SR355_ERR_INVALID;

@@ -212,36 +212,32 @@ __device__ __forceinline__ void tok_keep8(void *at16, unsigned char *at8, long l
         tok_v4u high;
         tok_v2u low;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const unsigned b0 = __builtin_bit_cast(unsigned, v[2 * j]), b1 = __builtin_bit_cast(unsigned, v[2 * j + 1]);
-            high[j] = (b0 >> 16) | (b1 & 0xffff0000u);
-        }
+        for (int j = 0; j < 4; ++j)                         // the upper halves of two values
+            high[j] = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, v[2 * j + 1]), __builtin_bit_cast(unsigned, v[2 * j]), 0x07060302u);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            unsigned w = 0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) w |= (__builtin_bit_cast(unsigned, v[4 * j + k]) >> 8 & 0xffu) << (8 * k);
-            low[j] = w;
-        }
+        for (int j = 0; j < 2; ++j)                         // byte 1 of four values
+            low[j] = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, v[4 * j + 1]), __builtin_bit_cast(unsigned, v[4 * j]), 0x0c0c0501u) |
+                     __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, v[4 * j + 3]), __builtin_bit_cast(unsigned, v[4 * j + 2]), 0x05010c0cu);
         *reinterpret_cast<tok_v4u *>((unsigned short *)at16 + at) = high;
         *reinterpret_cast<tok_v2u *>(at8 + at) = low;
     }
 }
 template <typename T>
-__device__ __forceinline__ void tok_kept8(const void *at16, const unsigned char *at8, long long at, float (&v)[8]) {
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int j = 0; j < 8; j += 4) tok_load<float, 4>((const float *)at16 + at + j, *reinterpret_cast<float(*)[4]>(v + j));
-    } else {
-        const tok_v4u high = *reinterpret_cast<const tok_v4u *>((const unsigned short *)at16 + at);
-        const tok_v2u low = *reinterpret_cast<const tok_v2u *>(at8 + at);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const unsigned h = j & 1 ? high[j / 2] & 0xffff0000u : high[j / 2] << 16;
-            v[j] = __builtin_bit_cast(float, h | (low[j / 4] >> (8 * (j & 3)) & 0xffu) << 8);
+struct TokKept8 {
+    tok_v4u high, more;                 // (fp32: two units)
+    tok_v2u low;
+    __device__ __forceinline__ void load(const void *at16, const unsigned char *at8, long long at) {
+        if constexpr (sizeof(T) == 4) {
+            high = *reinterpret_cast<const tok_v4u *>((const float *)at16 + at), more = *reinterpret_cast<const tok_v4u *>((const float *)at16 + at + 4);
+        } else {
+            high = *reinterpret_cast<const tok_v4u *>((const unsigned short *)at16 + at), low = *reinterpret_cast<const tok_v2u *>(at8 + at);
         }
     }
-}
+    __device__ __forceinline__ float value(int j) const {
+        if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, j < 4 ? high[j & 3] : more[j & 3]);
+        return __builtin_bit_cast(float, __builtin_amdgcn_perm(high[j / 2], low[j / 4], (j & 1 ? 0x0706000cu : 0x0504000cu) | (j & 3) << 8));
+    }
+};
 
 // Eight consecutive elements, in 16-byte accesses.
 template <typename T>
@@ -587,6 +583,36 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
     // rows [r of the turned fragments], all of this lane's columns
     auto finish = [&](auto kind, long long m_first) {
         constexpr int KIND = decltype(kind)::value;
+        if constexpr (EPI == TOK_EPI_GLU_GRAD) {
+            // UN rows' kept factors in flight: a load behind a store that it might alias waits for nothing else, but is not
+            // moved in front of it
+            constexpr int UN = 8;
+            static_assert(G::TURN * 32 % (ROWS * UN) == 0, "whole groups of rows");
+            for (int r0 = lane / LANES; r0 < G::TURN * 32; r0 += ROWS * UN) {
+                TokKept8<T> ka[UN], kd[UN];
+#pragma unroll
+                for (int k = 0; k < UN; ++k) {
+                    const long long m = m_first + r0 + k * ROWS;
+                    if (m >= job.M || !in_n) continue;
+                    ka[k].load(p.kept.a, p.kept.a_low, m * p.h_ld + n);
+                    kd[k].load(p.kept.d, p.kept.d_low, m * p.h_ld + n);
+                }
+#pragma unroll
+                for (int k = 0; k < UN; ++k) {
+                    const int r = r0 + k * ROWS;
+                    const long long m = m_first + r;
+                    if (m >= job.M || !in_n) continue;
+                    const tok_f32x4 lo = turned(r, col / 4), hi = turned(r, col / 4 + 1);
+                    const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                    float dg[8], du[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) dg[j] = v[j] * kd[k].value(j), du[j] = v[j] * ka[k].value(j);
+                    tok_store8<T>((T *)p.g + m * p.h_ld + n, dg);
+                    tok_store8<T>((T *)p.u + m * p.h_ld + n, du);
+                }
+            }
+            return;
+        }
 #pragma unroll 2
         for (int r = lane / LANES; r < G::TURN * 32; r += ROWS) {
             const long long m = m_first + r;
@@ -612,15 +638,6 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
                     for (int j = 0; j < 8; ++j) h[j] = tok_act<EXACT, KIND>(v[j] + bias[j]) * (w[j] + bias2[j]);
                 }
                 tok_store8<T>((T *)p.h + at, h);
-            } else if constexpr (EPI == TOK_EPI_GLU_GRAD) {
-                const long long at = m * p.h_ld + n;
-                float a[8], d[8];
-                tok_kept8<T>(p.kept.a, p.kept.a_low, at, a);
-                tok_kept8<T>(p.kept.d, p.kept.d_low, at, d);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) d[j] *= v[j], a[j] *= v[j];
-                tok_store8<T>((T *)p.g + at, d);
-                tok_store8<T>((T *)p.u + at, a);
             } else if constexpr (EPI == TOK_EPI_PART) {
                 float *part = job.part + ((size_t)split * job.M + m) * job.N + n;
                 if constexpr (KIND == WIDE) {

@@ -237,6 +237,7 @@ Tensor dropout_fwd(const Tensor &x, const OptTensor &skip, double p, const Tenso
     const Tensor r = x.contiguous();
     Launch launch(x);
     Tensor y = at::empty(x.sizes(), x.options());
+    if (x.numel() == 0) return y;
     ok(api.dropout(r.const_data_ptr(), ptr(s), x.numel(), code_of(x.scalar_type()), p, reinterpret_cast<const long long *>(rng.const_data_ptr()),
                    static_cast<unsigned>(site), y.mutable_data_ptr(), launch.stream),
        "sr355_dropout");

@@ -92,7 +92,7 @@ def test_c_entries_refuse_bad_arguments_without_touching_a_device(L):
     assert L.sr355_dropout(p, None, 8, F, float("nan"), p, 0, p, None) == -1
     assert L.sr355_dropout(p, None, 8, F, 0.5, None, 0, p, None) == -1
     assert L.sr355_dropout(p, None, -1, F, 0.5, p, 0, p, None) == -1
-    assert L.sr355_dropout(None, None, 0, F, 0.5, None, 0, None, None) == 0
+    assert L.sr355_dropout(p, None, 0, F, 0.5, p, 0, p, None) == -1
 
     def ffn(**kw):
         a = FfnArgs()
