@@ -74,11 +74,19 @@ __global__ __launch_bounds__(256) void reduce_splits_kernel(ReduceArgs a) {
     for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (long long)gridDim.x * 1024) {
         float v[4] = {0.f, 0.f, 0.f, 0.f};
         if (vec) {
-            for (int s = 0; s < a.splits; ++s) {
-                float t[4];
-                tok_load<float, 4>(part + (size_t)s * n + i, t);
+            // eight parts in flight (one after the other 32 parts of a small product took 10 us)
+            for (int s = 0; s < a.splits; s += 8) {
+                float t[8][4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] += t[j];
+                for (int k = 0; k < 8; ++k) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) t[k][j] = 0.f;
+                    if (s + k < a.splits) tok_load<float, 4>(part + (size_t)(s + k) * n + i, t[k]);
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] += t[k][j];
             }
             if (a.bias) {
 #pragma unroll
@@ -268,6 +276,13 @@ struct Saved {
     }
 };
 
+// Down of few rows: that kernel's workgroups each read all rows, 16 or fewer channels' worth, so with many rows and channels
+// the split product of 128-row tiles is faster (bf16, 2048 x 8192: 16 rows 14 against 15 us, 32 rows 22 against 15, 64 rows 37
+// against 17; 1024 x 4096: 8, 12 and 19 against 10, 10 and 12).  fp32 tiles are bound by the matrix pipes even then.
+bool few_down(const sr355_ffn_args *a) {
+    return a->rows <= 16 || (a->rows <= FEW_ROWS && (a->dtype == SR355_DTYPE_F32 || (long long)a->channels * a->hidden <= (1 << 21)));
+}
+
 struct ForwardPlan : Plan {
     Operand x, wg, wu, wd;
     TokKept kept = {};
@@ -292,7 +307,7 @@ struct ForwardPlan : Plan {
             return;
         }
         if (!h) h = take(hidden_bytes(a));
-        if (a->rows > FEW_ROWS) {
+        if (!few_down(a)) {
             down = product_splits(a->rows, a->channels, a->hidden, 1, a->dtype);
             if (down.n > 1) parts = (float *)take((size_t)down.n * a->rows * a->channels * sizeof(float));
             split = down.n > 1;
@@ -382,28 +397,31 @@ int few_rows(TokRowsArgs a, const char *what, hipStream_t stream) {
     hipLaunchKernelGGL((tok_rows_kernel<T, TG, GLU, WAVES>), dim3((unsigned)tok_cdiv(a.n_store, a.channels)), dim3(64 * WAVES), 0, stream, a);
     return check_hip(hipGetLastError(), what);
 }
-template <typename T, int TG>
-int few_rows_both(const TokRowsArgs &glu, const TokRowsArgs &down, hipStream_t stream) {
-    const int rc = few_rows<T, TG, true, TG == 4 ? 4 : 8>(glu, "gated_ffn gate / up launch", stream);
-    return rc != SR355_OK ? rc : few_rows<T, TG, false, TG == 4 ? 8 : 16>(down, "gated_ffn down launch", stream);
+template <typename T, bool GLU>
+int few_rows_any(const TokRowsArgs &a, const char *what, hipStream_t stream) {
+    if (a.rows <= 16) return few_rows<T, 1, GLU, GLU ? 8 : 16>(a, what, stream);
+    if (a.rows <= 32) return few_rows<T, 2, GLU, GLU ? 8 : 16>(a, what, stream);
+    return few_rows<T, 4, GLU, GLU ? 4 : 8>(a, what, stream);
 }
 
 template <typename T>
-int ffn_forward_few(const sr355_ffn_args *a, const ForwardPlan &p, hipStream_t stream) {
+int ffn_glu_few(const sr355_ffn_args *a, const ForwardPlan &p, hipStream_t stream) {
     TokRowsArgs g = {};
     g.x = (const unsigned char *)p.x.p, g.x_ld = p.x.ld * sizeof(T);
     g.w = (const unsigned char *)p.wg.p, g.w2 = (const unsigned char *)p.wu.p, g.w_ld = p.wg.ld * sizeof(T);
     g.rows = (int)a->rows, g.N = a->hidden, g.k_bytes = (int)(a->channels * sizeof(T));
     g.bias = a->b_gate_dev, g.bias2 = a->b_up_dev, g.act = a->activation;
     g.out = p.h, g.kept = p.kept, g.out_ld = hidden_ld(a), g.n_store = (int)hidden_ld(a);
+    return few_rows_any<T, true>(g, "gated_ffn gate / up launch", stream);
+}
+template <typename T>
+int ffn_down_few(const sr355_ffn_args *a, const ForwardPlan &p, hipStream_t stream) {
     TokRowsArgs d = {};
     d.x = (const unsigned char *)p.h, d.x_ld = hidden_ld(a) * sizeof(T);
     d.w = (const unsigned char *)p.wd.p, d.w_ld = p.wd.ld * sizeof(T);
     d.rows = (int)a->rows, d.N = a->channels, d.k_bytes = (int)(a->hidden * sizeof(T)), d.bias = a->b_down_dev;
     d.out = a->y_dev, d.out_ld = a->channels, d.n_store = a->channels;
-    if (a->rows <= 16) return few_rows_both<T, 1>(g, d, stream);
-    if (a->rows <= 32) return few_rows_both<T, 2>(g, d, stream);
-    return few_rows_both<T, 4>(g, d, stream);
+    return few_rows_any<T, false>(d, "gated_ffn down launch", stream);
 }
 
 template <typename T, int CP, int KIND>
@@ -441,7 +459,6 @@ int ffn_forward(const sr355_ffn_args *a, hipStream_t stream) {
     if constexpr (sizeof(T) == 2) {
         if (narrow_fits(a)) return ffn_forward_narrow<T>(a, p, stream);
     }
-    if (a->rows <= FEW_ROWS) return ffn_forward_few<T>(a, p, stream);
     TokGemmArgs g = {};
     g.n_jobs = 1, g.sections = 1, g.act = a->activation, g.K = a->channels;
     TokJob &j = g.job[0];
@@ -449,8 +466,9 @@ int ffn_forward(const sr355_ffn_args *a, hipStream_t stream) {
     j.b[0] = (const unsigned char *)p.wg.p, j.b[1] = (const unsigned char *)p.wu.p, j.b_ld = p.wg.ld * sizeof(T);
     j.M = (int)a->rows, j.N = a->hidden, j.bias = a->b_gate_dev;
     g.bias_up = a->b_up_dev, g.kept = p.kept, g.h = p.h, g.h_ld = hidden_ld(a);
-    rc = gemm_pick<T, false, false, TOK_EPI_GLU>(g, "gated_ffn gate / up launch", stream);
+    rc = a->rows <= FEW_ROWS ? ffn_glu_few<T>(a, p, stream) : gemm_pick<T, false, false, TOK_EPI_GLU>(g, "gated_ffn gate / up launch", stream);
     if (rc != SR355_OK) return rc;
+    if (few_down(a)) return ffn_down_few<T>(a, p, stream);
     TokGemmArgs d = {};
     d.n_jobs = 1, d.sections = 1, d.K = a->hidden;
     TokJob &k = d.job[0];
