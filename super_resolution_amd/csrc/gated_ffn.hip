@@ -17,7 +17,7 @@
 namespace sr355 {
 
 namespace {
-// 256 x 256 tiles where they fill the chip, one workgroup per CU; else 128 x 128, two per CU.  A row's share of a stage is a
+// 256 x 256 tiles, one workgroup per CU, or 128 x 128, two per CU (tiles_are_big).  A row's share of a stage is a
 // whole 128-byte line where k is contiguous (with 64 bytes every line comes twice from the L2: 147 against 138 us for
 // 16384 x 4096 times 4096 x 1024); where k is strided a stage's rows are lines in any case, and five stages of 64 bytes hide
 // more latency than two of 128 (443 against 472 us for the three weight gradients of 16384 x 1024 x 4096).
@@ -56,52 +56,53 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs p) {
     }
 }
 
-// out[j] = sum over splits, in order, of part[s * n + j]
-struct ReduceArgs {
-    const float *part[6];
-    void *out[6];
-    long long n[6];
-    int splits;
-    const void *bias;        // of columns (job 0), may be null
+// out[row][col] = sum over splits, in order, of part[s][row][col]; rows of the parts are whole groups of eight columns
+struct ReduceJob {
+    const float *part;
+    void *out;
+    long long rows;
     int cols;
+};
+struct ReduceArgs {
+    ReduceJob job[6];
+    int splits;
+    const void *bias;        // of columns, may be null
 };
 template <typename T>
 __global__ __launch_bounds__(256) void reduce_splits_kernel(ReduceArgs a) {
-    const float *part = a.part[blockIdx.y];
-    T *out = (T *)a.out[blockIdx.y];
-    const long long n = a.n[blockIdx.y];
-    const bool vec = (n & 3) == 0 && ((size_t)out & 15) == 0;
+    const ReduceJob &job = a.job[blockIdx.y];
+    const float *part = job.part;
+    const int cols = job.cols, ld = (cols + 7) & ~7;
+    const long long n = job.rows * ld;
+    const bool vec = cols == ld && ((size_t)job.out & 15) == 0;
     for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (long long)gridDim.x * 1024) {
         float v[4] = {0.f, 0.f, 0.f, 0.f};
+        // eight parts in flight (one after the other 32 parts of a small product took 10 us)
+        for (int s = 0; s < a.splits; s += 8) {
+            float t[8][4];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) t[k][j] = 0.f;
+                if (s + k < a.splits) tok_load<float, 4>(part + (size_t)(s + k) * n + i, t[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] += t[k][j];
+        }
+        const long long row = n <= 0x7fffffff ? (unsigned)i / (unsigned)ld : i / ld;
+        const int col = (int)(i - row * ld);
+        T *out = (T *)job.out + row * cols + col;
+        T o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = (T)(v[j] + (a.bias && col + j < cols ? (float)((const T *)a.bias)[col + j] : 0.f));
         if (vec) {
-            // eight parts in flight (one after the other 32 parts of a small product took 10 us)
-            for (int s = 0; s < a.splits; s += 8) {
-                float t[8][4];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) t[k][j] = 0.f;
-                    if (s + k < a.splits) tok_load<float, 4>(part + (size_t)(s + k) * n + i, t[k]);
-                }
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j] += t[k][j];
-            }
-            if (a.bias) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] += (float)((const T *)a.bias)[(i + j) % a.cols];
-            }
-            T o[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] = (T)v[j];
-            __builtin_memcpy(__builtin_assume_aligned(out + i, 4 * sizeof(T)), o, 4 * sizeof(T));
+            __builtin_memcpy(__builtin_assume_aligned(out, 4 * sizeof(T)), o, 4 * sizeof(T));
         } else {
-            for (int j = 0; j < 4 && i + j < n; ++j) {
-                for (int s = 0; s < a.splits; ++s) v[j] += part[(size_t)s * n + i + j];
-                if (a.bias) v[j] += (float)((const T *)a.bias)[(i + j) % a.cols];
-                out[i + j] = (T)v[j];
-            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (col + j < cols) out[j] = o[j];
         }
     }
 }
@@ -131,11 +132,18 @@ long long set_tiles(TokGemmArgs &g, bool glu) {
     return n;
 }
 
+// Which tiles take less: a CU works on one big or two small ones at a time, a quarter as much work each, and a round of big
+// ones takes 0.85 of two rounds of small ones for the halved operand traffic (bf16, 1024 x 4096, gate / up, big against small
+// tiles: 1500 rows 35 against 39 us, 4096 rows 83 against 98, 12000 rows 255 against 304).  What decides else is how full the
+// last round is (3000 rows, 384 big or 1536 small tiles: 70 against 67; down of 20000 rows, 316 or 1256: 235 against 219).
+bool tiles_are_big(long long big, long long small) { return 1.7 * tok_cdiv(big, N_CU) <= tok_cdiv(small, 2 * N_CU); }
+
 template <typename T, bool A_RC, bool B_RC, int EPI>
 int gemm_pick(TokGemmArgs &g, const char *what, hipStream_t stream) {
     g.splits = 1;
     const bool glu = EPI == TOK_EPI_GLU;
-    if (set_tiles<Tile256>(g, glu) >= N_CU) return gemm_launch<T, Tile256, A_RC, B_RC, EPI>(g, what, stream);
+    const long long small = set_tiles<Tile128>(g, glu);
+    if (tiles_are_big(set_tiles<Tile256>(g, glu), small)) return gemm_launch<T, Tile256, A_RC, B_RC, EPI>(g, what, stream);
     if (set_tiles<Tile128>(g, glu) > 0x3fffffffLL) {
         set_error("%s: too many tiles", what);
         return SR355_ERR_INVALID;
@@ -169,7 +177,9 @@ double stage_us(int dtype) {
 }
 
 // A product of rows and weights, split over k where its tiles are few; `parts` null: not split.
-bool product_is_big(long long rows, int n) { return tok_cdiv(rows, Tile256::BM) * tok_cdiv(n, Tile256::BN) >= N_CU; }
+bool product_is_big(long long rows, int n) {
+    return tiles_are_big(tok_cdiv(rows, Tile256::BM) * tok_cdiv(n, Tile256::BN), tok_cdiv(rows, Tile128::BM) * tok_cdiv(n, Tile128::BN));
+}
 Splits product_splits(long long rows, int n, int k, int sections, int dtype) {
     if (product_is_big(rows, n)) return {1, 0};
     const long long tiles = tok_cdiv(rows, Tile128::BM) * tok_cdiv(n, Tile128::BN);
@@ -180,8 +190,10 @@ Splits product_splits(long long rows, int n, int k, int sections, int dtype) {
 template <typename T>
 int reduce_launch(const ReduceArgs &r, int n_jobs, const char *what, hipStream_t stream) {
     long long most = 0;
-    for (int i = 0; i < n_jobs; ++i)
-        if (r.n[i] > most) most = r.n[i];
+    for (int i = 0; i < n_jobs; ++i) {
+        const long long n = r.job[i].rows * round_up(r.job[i].cols, 8);
+        if (n > most) most = n;
+    }
     const long long wgs = tok_cdiv(most, 1024);
     hipLaunchKernelGGL((reduce_splits_kernel<T>), dim3((unsigned)(wgs > 2048 ? 2048 : wgs), n_jobs), dim3(256), 0, stream, r);
     return check_hip(hipGetLastError(), what);
@@ -197,11 +209,18 @@ int product_launch(TokGemmArgs &g, const Splits &split, float *parts, const char
     const int rc = gemm_launch<T, Tile128, false, B_RC, TOK_EPI_PART>(g, what, stream);
     if (rc != SR355_OK) return rc;
     ReduceArgs r = {};
-    r.part[0] = parts, r.out[0] = j.c, r.n[0] = (long long)j.M * j.N, r.splits = split.n, r.bias = j.bias, r.cols = j.N;
+    r.job[0] = {parts, j.c, j.M, j.N}, r.splits = split.n, r.bias = j.bias;
     return reduce_launch<T>(r, 1, what, stream);
 }
 
 // ---- the plan of a call: what is copied, where things lie in the workspace --------------------------------------------
+// The row stride, in elements, of a buffer of this file's own: wide rows begin with a line of memory, or a stage's share of a
+// row is in two (fp16, 5003 x 501 x 1333, strides 512 and 1344 against 504 and 1336: down 21 against 26 us, gate / up 35
+// against 39).
+long long row_ld(int cols, int dtype) {
+    const int line = 128 / (int)tok_type_bytes(dtype);
+    return round_up(cols, cols >= 4 * line ? line : 8);
+}
 struct Operand {
     const void *p;
     long long ld;     // elements
@@ -222,7 +241,7 @@ struct Plan {
         const int e = dtype == SR355_DTYPE_F32 ? 4 : 8;
         const long long row_bytes = ld * (long long)tok_type_bytes(dtype);
         if (cols % e == 0 && ld % e == 0 && tok_aligned16(p) && row_bytes < (1LL << 22)) return {p, ld};
-        const long long dst_ld = round_up(cols, e);
+        const long long dst_ld = row_ld(cols, dtype);
         void *dst = take((size_t)rows * dst_ld * tok_type_bytes(dtype));
         pads.job[n_pads++] = {p, dst, rows, ld, dst_ld, cols};
         return {dst, dst_ld};
@@ -243,8 +262,10 @@ int run_pads(const Plan &plan, hipStream_t stream) {
     return check_hip(hipGetLastError(), "gated_ffn row padding launch");
 }
 
-// rows of g, u, h, dg, du: whole groups of eight channels, what a lane of the epilogue stores
-long long hidden_ld(const sr355_ffn_args *a) { return round_up(a->hidden, 8); }
+// Rows of h, the kept factors, dg and du: whole groups of eight channels, what a lane of the epilogue stores (zeros behind the
+// last channel); wide ones begin with a line of memory.
+long long hidden_cols(const sr355_ffn_args *a) { return round_up(a->hidden, 8); }
+long long hidden_ld(const sr355_ffn_args *a) { return row_ld(a->hidden, a->dtype); }
 
 size_t hidden_bytes(const sr355_ffn_args *a) {
     return ((size_t)a->rows * hidden_ld(a) * tok_type_bytes(a->dtype) + 255) & ~(size_t)255;
@@ -302,14 +323,14 @@ struct ForwardPlan : Plan {
             kept = s.kept, h = s.h;
         }
         if (narrow_fits(a)) {
-            if (a->b_gate_dev) bg = operand(a->b_gate_dev, 1, a->hidden, hidden_ld(a), a->dtype);
-            if (a->b_up_dev) bu = operand(a->b_up_dev, 1, a->hidden, hidden_ld(a), a->dtype);
+            if (a->b_gate_dev) bg = operand(a->b_gate_dev, 1, a->hidden, hidden_cols(a), a->dtype);
+            if (a->b_up_dev) bu = operand(a->b_up_dev, 1, a->hidden, hidden_cols(a), a->dtype);
             return;
         }
         if (!h) h = take(hidden_bytes(a));
         if (!few_down(a)) {
             down = product_splits(a->rows, a->channels, a->hidden, 1, a->dtype);
-            if (down.n > 1) parts = (float *)take((size_t)down.n * a->rows * a->channels * sizeof(float));
+            if (down.n > 1) parts = (float *)take((size_t)down.n * a->rows * round_up(a->channels, 8) * sizeof(float));
             split = down.n > 1;
         }
     }
@@ -366,13 +387,13 @@ struct BackwardPlan : Plan {
         dg = need_hidden ? take(hidden_bytes(a)) : nullptr;
         du = need_hidden ? take(hidden_bytes(a)) : nullptr;
         wgrad = wgrad_shape(a);
-        const size_t mats = (a->dw_gate_dev != nullptr) + (a->dw_up_dev != nullptr) + (a->dw_down_dev != nullptr);
-        parts = mats && wgrad.split.n > 1
-                    ? (float *)take(mats * wgrad.split.n * (size_t)a->hidden * a->channels * sizeof(float)) : nullptr;
+        const size_t wide = (size_t)a->hidden * round_up(a->channels, 8), tall = (size_t)a->channels * round_up(a->hidden, 8);
+        const size_t sums = (a->dw_gate_dev ? wide : 0) + (a->dw_up_dev ? wide : 0) + (a->dw_down_dev ? tall : 0);
+        parts = sums && wgrad.split.n > 1 ? (float *)take(wgrad.split.n * sums * sizeof(float)) : nullptr;
         dx = {1, 0};
         if (a->dx_dev && a->rows > 0) dx = product_splits(a->rows, a->channels, a->hidden, 2, a->dtype);
-        dx_parts = dx.n > 1 ? (float *)take((size_t)dx.n * a->rows * a->channels * sizeof(float)) : nullptr;
-        row_parts = wgrad.split.n > 1 ? (float *)take((size_t)wgrad.split.n * (2 * (size_t)a->hidden + a->channels) * sizeof(float)) : nullptr;
+        dx_parts = dx.n > 1 ? (float *)take((size_t)dx.n * a->rows * round_up(a->channels, 8) * sizeof(float)) : nullptr;
+        row_parts = wgrad.split.n > 1 ? (float *)take((size_t)wgrad.split.n * (2 * round_up(a->hidden, 8) + round_up(a->channels, 8)) * sizeof(float)) : nullptr;
     }
 };
 
@@ -411,7 +432,7 @@ int ffn_glu_few(const sr355_ffn_args *a, const ForwardPlan &p, hipStream_t strea
     g.w = (const unsigned char *)p.wg.p, g.w2 = (const unsigned char *)p.wu.p, g.w_ld = p.wg.ld * sizeof(T);
     g.rows = (int)a->rows, g.N = a->hidden, g.k_bytes = (int)(a->channels * sizeof(T));
     g.bias = a->b_gate_dev, g.bias2 = a->b_up_dev, g.act = a->activation;
-    g.out = p.h, g.kept = p.kept, g.out_ld = hidden_ld(a), g.n_store = (int)hidden_ld(a);
+    g.out = p.h, g.kept = p.kept, g.out_ld = hidden_ld(a), g.n_store = (int)hidden_cols(a);
     return few_rows_any<T, true>(g, "gated_ffn gate / up launch", stream);
 }
 template <typename T>
@@ -491,7 +512,6 @@ int ffn_wgrad(const sr355_ffn_args *a, const BackwardPlan &p, hipStream_t stream
     g.sections = 1, g.K = (int)a->rows, g.splits = p.wgrad.split.n, g.split_stages = p.wgrad.split.stages;
     ReduceArgs r = {};
     float *parts = p.parts, *row_parts = p.row_parts;
-    const size_t n = (size_t)a->hidden * a->channels;
     int n_out = 0;
     auto add = [&](const void *l, long long l_ld, const void *q, long long q_ld, int M, int N, void *out, void *sums) {
         if (!out && !sums) return;
@@ -501,12 +521,12 @@ int ffn_wgrad(const sr355_ffn_args *a, const BackwardPlan &p, hipStream_t stream
         j.M = M, j.N = out ? N : 1, j.c = out, j.c_ld = N, j.row_sums = sums;
         if (g.splits == 1) return;
         if (out) {
-            j.part = parts, parts += g.splits * n;
-            r.part[n_out] = j.part, r.out[n_out] = out, r.n[n_out++] = (long long)n;
+            j.part = parts, parts += (size_t)g.splits * M * round_up(N, 8);
+            r.job[n_out++] = {j.part, out, M, N};
         }
         if (sums) {
-            j.row_part = row_parts, row_parts += (size_t)g.splits * M;
-            r.part[n_out] = j.row_part, r.out[n_out] = sums, r.n[n_out++] = M;
+            j.row_part = row_parts, row_parts += (size_t)g.splits * round_up(M, 8);
+            r.job[n_out++] = {j.row_part, sums, 1, M};
         }
     };
     add(p.dg, hidden_ld(a), p.x.p, p.x.ld, a->hidden, a->channels, a->dw_gate_dev, a->db_gate_dev);

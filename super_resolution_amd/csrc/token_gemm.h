@@ -54,9 +54,9 @@ struct TokJob {
     void *c;
     long long c_ld;                     // elements
     const void *bias;                   // [N] of T, may be null
-    float *part;                        // split products: [splits][M][N] fp32 partials
+    float *part;                        // split products: [splits][M][N rounded up to 8] fp32 partials
     void *row_sums;                     // A strided in k: [M] of T, sums of A over k (may be null; c may be null with it)
-    float *row_part;                    // split products: [splits][M] fp32 partials of them
+    float *row_part;                    // split products: [splits][M rounded up to 8] fp32 partials of them
     int tiles_m, tiles_n;
 };
 struct TokGemmArgs {
@@ -553,7 +553,7 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
                 const float s = row_sum[i] + __shfl_xor(row_sum[i], 32, 64);
                 const long long m = m0 + (wm * MT + i) * 32 + (lane & 31);
                 if (lane < 32 && m < job.M) {
-                    if constexpr (EPI == TOK_EPI_PART) job.row_part[(size_t)split * job.M + m] = s;
+                    if constexpr (EPI == TOK_EPI_PART) job.row_part[(size_t)split * ((job.M + 7) & ~7) + m] = s;
                     else ((T *)job.row_sums)[m] = (T)s;
                 }
             }
@@ -569,9 +569,11 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
     auto turned = [&](int r, int chunk) -> tok_f32x4 {
         return *reinterpret_cast<const tok_f32x4 *>(turn + (r * CHUNKS + (chunk ^ (r % CHUNKS))) * 16);
     };
-    // results without an activation go out 16 bytes at a time where their rows allow it
+    // Results in rows of whole, aligned units go out 16 bytes a lane (all but a STORE's are laid out so, with zeros up to the
+    // next eighth column); others one row of the wave's columns an instruction, one element a lane.
     constexpr int NARROW = 0, WIDE = 1;
-    const bool wide = (job.N & 7) == 0 && (EPI == TOK_EPI_PART || ((job.c_ld & 7) == 0 && ((size_t)job.c & 15) == 0));
+    const bool wide = EPI != TOK_EPI_STORE || ((job.N & 7) == 0 && (job.c_ld & 7) == 0 && ((size_t)job.c & 15) == 0);
+    const int n_stored = EPI == TOK_EPI_STORE ? job.N : (job.N + 7) & ~7;
     float bias[8], bias2[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -579,7 +581,7 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
         bias[j] = (EPI == TOK_EPI_GLU || EPI == TOK_EPI_STORE) && job.bias && n + j < job.N ? (float)((const T *)job.bias)[n + j] : 0.f;
         bias2[j] = EPI == TOK_EPI_GLU && p.bias_up && n + j < job.N ? (float)((const T *)p.bias_up)[n + j] : 0.f;
     }
-    const bool in_n = n < (EPI == TOK_EPI_GLU || EPI == TOK_EPI_GLU_GRAD ? p.h_ld : (long long)job.N);
+    const bool in_n = n < n_stored;
     // rows [r of the turned fragments], all of this lane's columns
     auto finish = [&](auto kind, long long m_first) {
         constexpr int KIND = decltype(kind)::value;
@@ -613,6 +615,17 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
             }
             return;
         }
+        if constexpr (EPI == TOK_EPI_STORE && KIND == NARROW) {
+            static_assert(COLS == 64, "a lane per column");
+            const int n1 = n0 + wn * COLS + lane;
+            if (n1 >= job.N) return;
+            const float b = job.bias ? (float)((const T *)job.bias)[n1] : 0.f;
+            const int rows = job.M - m_first < G::TURN * 32 ? (int)(job.M - m_first) : G::TURN * 32;
+            T *c = (T *)job.c + m_first * job.c_ld + n1;
+#pragma unroll 4
+            for (int r = 0; r < rows; ++r) c[r * job.c_ld] = (T)(turned(r, lane / 4)[lane & 3] + b);
+            return;
+        }
 #pragma unroll 2
         for (int r = lane / LANES; r < G::TURN * 32; r += ROWS) {
             const long long m = m_first + r;
@@ -639,25 +652,11 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
                 }
                 tok_store8<T>((T *)p.h + at, h);
             } else if constexpr (EPI == TOK_EPI_PART) {
-                float *part = job.part + ((size_t)split * job.M + m) * job.N + n;
-                if constexpr (KIND == WIDE) {
-                    tok_store8<float>(part, v);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (n + j < job.N) part[j] = v[j];
-                }
+                tok_store8<float>(job.part + ((size_t)split * job.M + m) * n_stored + n, v);
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] += bias[j];
-                T *c = (T *)job.c + m * job.c_ld + n;
-                if constexpr (KIND == WIDE) {
-                    tok_store8<T>(c, v);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (n + j < job.N) c[j] = (T)v[j];
-                }
+                tok_store8<T>((T *)job.c + m * job.c_ld + n, v);
             }
         }
     };
@@ -685,7 +684,7 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
             else if (p.act == SR355_ACT_RELU) finish(std::integral_constant<int, SR355_ACT_RELU>{}, m_first);
             else finish(std::integral_constant<int, SR355_ACT_SIGMOID>{}, m_first);
         } else {
-            if (EPI == TOK_EPI_GLU_GRAD || wide) finish(std::integral_constant<int, WIDE>{}, m_first);
+            if (wide) finish(std::integral_constant<int, WIDE>{}, m_first);
             else finish(std::integral_constant<int, NARROW>{}, m_first);
         }
     }
