@@ -43,7 +43,8 @@ def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, b_gate: O
     """``(act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down`` for rows ``x`` ``[..., C]``, ``w_gate`` and
     ``w_up`` ``[F, C]`` and ``w_down`` ``[C, F]`` (``nn.Linear`` weights), all of x's type.  ``activation``: "silu", "gelu"
     (by the error function), "relu" or "sigmoid".  Products accumulate in fp32; the hidden channels are held in x's type
-    between the launches.  A call that autograd records keeps eight bytes (float32: twelve) per hidden channel of every row of x."""
+    between the launches.  A call that autograd records keeps eight bytes (float32: twelve) per
+    hidden channel of every row of x."""
     if activation not in ops.ACTIVATIONS:
         raise RuntimeError(f"gated_ffn: activation must be one of {', '.join(ops.ACTIVATIONS)}, got {activation!r}")
     return (ops._binding or ops.binding()).gated_ffn(x, w_gate, w_up, w_down, b_gate, b_up, b_down, ops.ACTIVATIONS[activation])
