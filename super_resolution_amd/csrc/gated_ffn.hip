@@ -17,7 +17,7 @@
 namespace sr355 {
 
 namespace {
-// 256 x 256 tiles, one workgroup per CU, or 128 x 128, two per CU (tiles_are_big).  A row's share of a stage is a
+// 16-bit types: 256 x 256 tiles, one workgroup per CU, or 128 x 128, two per CU (tiles_are_big).  A row's share of a stage is a
 // whole 128-byte line where k is contiguous (with 64 bytes every line comes twice from the L2: 147 against 138 us for
 // 16384 x 4096 times 4096 x 1024); where k is strided a stage's rows are lines in any case, and five stages of 64 bytes hide
 // more latency than two of 128 (443 against 472 us for the three weight gradients of 16384 x 1024 x 4096).
@@ -25,6 +25,21 @@ typedef TokTile<256, 256, 2, 4, 128, 2> Tile256;
 typedef TokTile<256, 256, 2, 4, 64, 5> TileWgrad;
 typedef TokTile<128, 128, 2, 2, 128, 2> Tile128;
 constexpr int N_CU = 256;
+
+// fp32: 32 x 32 x 2 instructions take eight times as long for the same bytes, so operand traffic does not matter and small tiles,
+// three workgroups per CU, hide starts and ends best (forward and backward kernels, 1000 x 256 x 1024: 102 us, with 128 x 128
+// tiles, two per CU, 128; 3001 x 501 x 1333: 438 and 474; 9000 x 1024 x 4096: 5473 and 5593, with 256 x 256 tiles 6502).
+typedef TokTile<128, 64, 4, 1, 128, 2> TileF32;
+template <typename T>
+using TileSmall = typename std::conditional<sizeof(T) == 4, TileF32, Tile128>::type;
+struct SmallShape {
+    int bm, bn, kb, slots;       // slots: workgroups of all CUs at a time
+    SmallShape(int dtype) {
+        if (dtype == SR355_DTYPE_F32) bm = TileF32::BM, bn = TileF32::BN, kb = TileF32::KB, slots = 3 * N_CU;
+        else bm = Tile128::BM, bn = Tile128::BN, kb = Tile128::KB, slots = 2 * N_CU;
+    }
+    long long tiles(long long m, long long n) const { return tok_cdiv(m, bm) * tok_cdiv(n, bn); }
+};
 
 struct PadJob {
     const void *src;
@@ -142,13 +157,15 @@ template <typename T, bool A_RC, bool B_RC, int EPI>
 int gemm_pick(TokGemmArgs &g, const char *what, hipStream_t stream) {
     g.splits = 1;
     const bool glu = EPI == TOK_EPI_GLU;
-    const long long small = set_tiles<Tile128>(g, glu);
-    if (tiles_are_big(set_tiles<Tile256>(g, glu), small)) return gemm_launch<T, Tile256, A_RC, B_RC, EPI>(g, what, stream);
-    if (set_tiles<Tile128>(g, glu) > 0x3fffffffLL) {
+    if constexpr (sizeof(T) == 2) {
+        const long long small = set_tiles<Tile128>(g, glu);
+        if (tiles_are_big(set_tiles<Tile256>(g, glu), small)) return gemm_launch<T, Tile256, A_RC, B_RC, EPI>(g, what, stream);
+    }
+    if (set_tiles<TileSmall<T>>(g, glu) > 0x3fffffffLL) {
         set_error("%s: too many tiles", what);
         return SR355_ERR_INVALID;
     }
-    return gemm_launch<T, Tile128, A_RC, B_RC, EPI>(g, what, stream);
+    return gemm_launch<T, TileSmall<T>, A_RC, B_RC, EPI>(g, what, stream);
 }
 
 // Into how many parts the sum over k of a few tiles is split: the number that takes least, by the rounds of the chip
@@ -171,20 +188,22 @@ Splits pick_splits(long long tiles, int slots, long long stages, double elements
 template <typename G>
 double stage_us(int dtype) {
     // MFMA cycles of a stage's workgroups on a CU (32 a 32 x 32 x 16, 64 a 32 x 32 x 2) at 2 GHz and 70 % of the pipes
-    const double wgs = G::LDS_BYTES > 80 * 1024 ? 1 : 2;
+    const double wgs = 160 * 1024 / G::LDS_BYTES;
     const double mfma = (double)G::MT * G::NT * G::KS * (dtype == SR355_DTYPE_F32 ? 4 * 64 : 32) * (G::WAVES / 4);
     return mfma * wgs / 2000.0 / 0.7;
 }
 
 // A product of rows and weights, split over k where its tiles are few; `parts` null: not split.
-bool product_is_big(long long rows, int n) {
-    return tiles_are_big(tok_cdiv(rows, Tile256::BM) * tok_cdiv(n, Tile256::BN), tok_cdiv(rows, Tile128::BM) * tok_cdiv(n, Tile128::BN));
+bool product_is_big(long long rows, int n, int dtype) {
+    return dtype != SR355_DTYPE_F32 &&
+           tiles_are_big(tok_cdiv(rows, Tile256::BM) * tok_cdiv(n, Tile256::BN), SmallShape(dtype).tiles(rows, n));
 }
 Splits product_splits(long long rows, int n, int k, int sections, int dtype) {
-    if (product_is_big(rows, n)) return {1, 0};
-    const long long tiles = tok_cdiv(rows, Tile128::BM) * tok_cdiv(n, Tile128::BN);
-    const long long stages = tok_cdiv(k, Tile128::KB / (long long)tok_type_bytes(dtype)) * sections;
-    return pick_splits(tiles, 2 * N_CU, stages, (double)rows * n, stage_us<Tile128>(dtype));
+    if (product_is_big(rows, n, dtype)) return {1, 0};
+    const SmallShape small(dtype);
+    const long long stages = tok_cdiv(k, small.kb / (long long)tok_type_bytes(dtype)) * sections;
+    return pick_splits(small.tiles(rows, n), small.slots, stages, (double)rows * n,
+                       dtype == SR355_DTYPE_F32 ? stage_us<TileF32>(dtype) : stage_us<Tile128>(dtype));
 }
 
 template <typename T>
@@ -205,8 +224,8 @@ int product_launch(TokGemmArgs &g, const Splits &split, float *parts, const char
     TokJob &j = g.job[0];
     g.splits = split.n, g.split_stages = split.stages;
     j.part = parts;
-    set_tiles<Tile128>(g, false);
-    const int rc = gemm_launch<T, Tile128, false, B_RC, TOK_EPI_PART>(g, what, stream);
+    set_tiles<TileSmall<T>>(g, false);
+    const int rc = gemm_launch<T, TileSmall<T>, false, B_RC, TOK_EPI_PART>(g, what, stream);
     if (rc != SR355_OK) return rc;
     ReduceArgs r = {};
     r.job[0] = {parts, j.c, j.M, j.N}, r.splits = split.n, r.bias = j.bias;
@@ -356,8 +375,9 @@ Splits wgrad_splits(const sr355_ffn_args *a, int slots) {
                        (double)mats * a->hidden * a->channels, stage_us<G>(a->dtype));
 }
 WgradShape wgrad_shape(const sr355_ffn_args *a) {
+    if (a->dtype == SR355_DTYPE_F32) return {false, wgrad_splits<TileF32>(a, SmallShape(a->dtype).slots)};
     if (wgrad_tiles<TileWgrad>(a) >= N_CU / 4) return {true, wgrad_splits<TileWgrad>(a, N_CU)};
-    return {false, wgrad_splits<Tile128>(a, 2 * N_CU)};
+    return {false, wgrad_splits<Tile128>(a, SmallShape(a->dtype).slots)};
 }
 
 struct BackwardPlan : Plan {
@@ -535,8 +555,13 @@ int ffn_wgrad(const sr355_ffn_args *a, const BackwardPlan &p, hipStream_t stream
     if (!g.n_jobs) return SR355_OK;
     const bool part = g.splits > 1;
     const bool sums = a->db_gate_dev || a->db_up_dev || a->db_down_dev;
-    const int rc = p.wgrad.big ? (sums ? wgrad_launch<T, TileWgrad, true>(g, part, stream) : wgrad_launch<T, TileWgrad, false>(g, part, stream))
-                               : (sums ? wgrad_launch<T, Tile128, true>(g, part, stream) : wgrad_launch<T, Tile128, false>(g, part, stream));
+    int rc;
+    if constexpr (sizeof(T) == 2) {
+        if (p.wgrad.big) rc = sums ? wgrad_launch<T, TileWgrad, true>(g, part, stream) : wgrad_launch<T, TileWgrad, false>(g, part, stream);
+        else rc = sums ? wgrad_launch<T, Tile128, true>(g, part, stream) : wgrad_launch<T, Tile128, false>(g, part, stream);
+    } else {
+        rc = sums ? wgrad_launch<T, TileF32, true>(g, part, stream) : wgrad_launch<T, TileF32, false>(g, part, stream);
+    }
     if (rc != SR355_OK || !part) return rc;
     r.splits = p.wgrad.split.n;
     return reduce_launch<T>(r, n_out, "gated_ffn weight gradient reduction launch", stream);

@@ -588,7 +588,7 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
         if constexpr (EPI == TOK_EPI_GLU_GRAD) {
             // UN rows' kept factors in flight: a load behind a store that it might alias waits for nothing else, but is not
             // moved in front of it
-            constexpr int UN = 8;
+            constexpr int UN = G::TURN * 32 / ROWS < 8 ? G::TURN * 32 / ROWS : 8;
             static_assert(G::TURN * 32 % (ROWS * UN) == 0, "whole groups of rows");
             for (int r0 = lane / LANES; r0 < G::TURN * 32; r0 += ROWS * UN) {
                 TokKept8<T> ka[UN], kd[UN];
