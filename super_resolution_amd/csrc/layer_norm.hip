@@ -13,6 +13,10 @@ namespace sr355 {
 namespace {
 constexpr int LN_THREADS = 256;
 constexpr int LN_MAX_PARTS = 512;      // two workgroups per CU
+constexpr int LN_LONG = 8192;          // channels from which on no type's row fits a workgroup's registers
+
+// Partial rows of dw and db, at most: rows beyond the registers have columns enough to fill the chip with fewer.
+int ln_max_parts(int C) { return C <= LN_LONG ? LN_MAX_PARTS : C <= 65536 ? 64 : 8; }
 
 // Sum over the lanes that hold one row.  L = 256: the four waves through LDS (red: 2 x 4 floats, alternating, so that
 // one barrier per sum is enough).
@@ -246,20 +250,20 @@ __global__ __launch_bounds__(LN_THREADS) void ln_bwd_long_kernel(LnArgs a) {
     }
 }
 
-// dw / db of long rows: workgroup (part, block of 256 columns), one column per thread.
+// dw / db of long rows: workgroup (block of 256 columns, part), one column per thread.
 template <typename T>
 __global__ __launch_bounds__(LN_THREADS) void ln_columns_long_kernel(LnArgs a) {
-    const int c = blockIdx.y * LN_THREADS + threadIdx.x;
+    const int c = blockIdx.x * LN_THREADS + threadIdx.x;
     if (c >= a.C) return;
     float sw = 0.f, sb = 0.f;
-    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    for (long long row = blockIdx.y; row < a.rows; row += gridDim.y) {
         const float d = (float)((const T *)a.dy)[row * a.dy_ld + c];
         sw += d * (((float)((const T *)a.x)[row * a.x_ld + c] - a.mean[row]) * a.rstd[row]);
         sb += d;
     }
-    float *part = a.parts + (size_t)blockIdx.x * 2 * a.C;
+    float *part = a.parts + (size_t)blockIdx.y * 2 * a.C;
     part[c] = sw;
-    part[a.C + c] = sb;
+    part[(size_t)a.C + c] = sb;
 }
 
 // out[k][j] = sum over parts p, in order, of parts[p * stride + first[k] + j]: the tail of every two-level column sum.
@@ -352,9 +356,9 @@ struct LnBackward {
     template <typename T>
     int run_long() {
         if (a.y) hipLaunchKernelGGL((ln_bwd_long_kernel<T>), dim3(ln_grid(a.rows, 1, 1 << 20)), dim3(LN_THREADS), 0, stream, a);
-        *n_parts = ln_grid(a.rows, 64, 64);
+        *n_parts = ln_grid(a.rows, 64, ln_max_parts(a.C) < 64 ? ln_max_parts(a.C) : 64);
         if (a.parts)
-            hipLaunchKernelGGL((ln_columns_long_kernel<T>), dim3(*n_parts, (unsigned)tok_cdiv(a.C, LN_THREADS)), dim3(LN_THREADS), 0,
+            hipLaunchKernelGGL((ln_columns_long_kernel<T>), dim3((unsigned)tok_cdiv(a.C, LN_THREADS), *n_parts), dim3(LN_THREADS), 0,
                                stream, a);
         return check_hip(hipGetLastError(), "layer_norm_bwd launch");
     }
@@ -425,7 +429,7 @@ size_t sr355_layer_norm_bwd_workspace_bytes(int C) {
         set_error("layer_norm_bwd_workspace_bytes: C=%d", C);
         return 0;
     }
-    return (size_t)LN_MAX_PARTS * 2 * C * sizeof(float);
+    return (size_t)ln_max_parts(C) * 2 * C * sizeof(float);
 }
 
 int sr355_layer_norm_bwd(const void *dy, long long dy_ld, const void *x, long long x_ld, long long rows, int C, int dtype,

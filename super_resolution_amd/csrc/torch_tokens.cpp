@@ -7,8 +7,10 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <array>
@@ -108,10 +110,27 @@ struct Launch {                       // the tensors' device is current and its 
 
 Tensor scratch(const Tensor &x, size_t bytes) { return at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte)); }
 
-bool recorded(std::initializer_list<const Tensor *> ts) {
+// A leaf's gradients are added up on the stream that was current when the oldest live graph of the leaf was recorded.  In a
+// capture that must not be the default stream: the engine would make it wait for the captured one, which ends the process.
+void check_capture(const std::vector<Tensor> &inputs) {
+    for (const Tensor &t : inputs) {
+        if (!t.defined() || !t.is_cuda() || !t.requires_grad() || !t.is_leaf()) continue;
+        const c10::OptionalDeviceGuard guard(t.device());
+        if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+        const auto stream = node ? node->stream() : std::nullopt;
+        TORCH_CHECK(!stream || stream->id() != 0, "a graph is being captured, and a leaf of shape ", t.sizes(),
+                    " still belongs to one that was recorded on the default stream: drop that graph's outputs first");
+    }
+}
+// whether autograd records a call with these inputs
+bool recorded(const std::vector<Tensor> &ts) {
     if (!at::GradMode::is_enabled()) return false;
-    for (const Tensor *t : ts)
-        if (t->defined() && t->requires_grad()) return true;
+    for (const Tensor &t : ts)
+        if (t.defined() && t.requires_grad()) {
+            check_capture(ts);
+            return true;
+        }
     return false;
 }
 Tensor defined(const OptTensor &t) { return t.has_value() ? *t : Tensor(); }
@@ -215,7 +234,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 Tensor layer_norm(const Tensor &x, const OptTensor &weight, const OptTensor &bias, double eps) {
     const Tensor w = defined(weight), b = defined(bias);
-    if (recorded({&x, &w, &b})) return LayerNorm::apply(x, weight, bias, eps);
+    if (recorded({x, w, b})) return LayerNorm::apply(x, weight, bias, eps);
     return std::get<0>(layer_norm_fwd(x, weight, bias, eps, false));
 }
 
@@ -264,7 +283,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 
 Tensor dropout(const Tensor &x, double p, const Tensor &rng, int64_t site, const OptTensor &residual) {
     const Tensor s = defined(residual);
-    if (recorded({&x, &s})) return Dropout::apply(x, p, rng, site, residual);
+    if (recorded({x, s})) return Dropout::apply(x, p, rng, site, residual);
     return dropout_fwd(x, residual, p, rng, site);
 }
 
@@ -376,7 +395,7 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
 Tensor gated_ffn(const Tensor &x, const Tensor &w_gate, const Tensor &w_up, const Tensor &w_down, const OptTensor &b_gate,
                  const OptTensor &b_up, const OptTensor &b_down, int64_t activation) {
     const Tensor bg = defined(b_gate), bu = defined(b_up), bd = defined(b_down);
-    if (recorded({&x, &w_gate, &w_up, &w_down, &bg, &bu, &bd}))
+    if (recorded({x, w_gate, w_up, w_down, bg, bu, bd}))
         return GatedFfn::apply(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation);
     return std::get<0>(gated_ffn_fwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation, false));
 }
@@ -387,6 +406,7 @@ PYBIND11_MODULE(_torch_tokens, m) {
     namespace py = pybind11;
     typedef py::call_guard<py::gil_scoped_release> free;
     m.def("connect", &connect);
+    m.def("check_capture", &check_capture);
     m.def("layer_norm", &layer_norm, free());
     m.def("dropout", &dropout, free());
     m.def("gated_ffn", &gated_ffn, free());

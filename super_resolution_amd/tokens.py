@@ -7,7 +7,8 @@ fp32 sums of a fixed order; ``FeedForwardBlock`` composes them into the channel-
 
 Any sizes, leading dimensions and strides are taken; what is not laid out as rows of contiguous channels is copied first.
 Widths that are multiples of 16 bytes are the fast ones.  All calls run on the current stream of their tensors' device, can
-be captured into a graph, and keep nothing between calls."""
+be captured into a graph, and keep nothing between calls.  A training call that is captured refuses leaves that a live
+autograd graph of the default stream still holds: PyTorch would add their gradients up there."""
 from __future__ import annotations
 
 from typing import Optional
@@ -76,7 +77,8 @@ class FeedForwardBlock(nn.Module):
     Parameters are float32; where x is bfloat16 or float16 the projections' are rounded to its type for the call (their
     gradients come back as float32) and the normalisation's are used as they are.  In training mode with ``dropout > 0``
     every call takes the seed and step of ``rng_state`` (a buffer that checkpoints carry; ``seed()`` sets it) and advances
-    the step, on the device, so that replays of a captured graph do too."""
+    the step, on the device, so that replays of a captured graph do too.  A forward pass that is run again for its gradients
+    (activation checkpointing) would take the next step and drop other elements: set ``rng_state`` back for it."""
 
     def __init__(self, channels: int, hidden: int, dropout: float = 0.0, activation: str = "silu", bias: bool = True,
                  eps: float = 1e-5):
@@ -98,6 +100,9 @@ class FeedForwardBlock(nn.Module):
     def forward(self, x: Tensor) -> Tensor:
         if x.dim() < 1 or x.shape[-1] != self.channels:
             raise RuntimeError(f"FeedForwardBlock: expected rows of {self.channels} channels, got {tuple(x.shape)}")
+
+        if torch.is_grad_enabled() and x.is_cuda:
+            ops.binding().check_capture([x, *self.parameters()])     # (the calls see the parameters' copies in x's type)
 
         def typed(t: Optional[Tensor]) -> Optional[Tensor]:
             return None if t is None else t.to(x.dtype)

@@ -109,6 +109,17 @@ def test_layer_norm_without_parameters_and_single_gradients(dtype):
     within(torch.autograd.grad(y, bg, dy)[0], dy.double().sum(0), tol[3] + half_step(dtype) * dy.double().sum(0).abs() + 1e-30)
 
 
+def test_layer_norm_of_rows_with_more_columns_than_a_grid_axis_has_blocks():
+    rows, c = 2, (1 << 24) + 5
+    x, dy = rnd(rows, c, seed=16), rnd(rows, c, seed=17)
+    w, b = rnd(c, seed=18), rnd(c, seed=19)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = tokens.layer_norm(*leaves)
+    got = (y, *torch.autograd.grad(y, leaves, dy))
+    for g, want, tol in zip(got, *norm_bounds(x.detach(), w.detach(), b.detach(), dy, 1e-5, B)):
+        within(g.detach(), want, tol + B * want.abs() + 1e-30)
+
+
 def test_layer_norm_strides_alignment_and_odd_rows():
     big = rnd(40, 300, seed=8)
     ref = lambda t: tokens.layer_norm(t.contiguous().clone())
@@ -581,6 +592,33 @@ def test_two_graphs_do_not_share_memory():
     torch.cuda.synchronize()
     for k in range(2):
         assert all(torch.equal(a, b) for a, b in zip(outs[k], chain(x * (k + 1), ws, rng, dy)))
+
+
+def test_a_capture_refuses_leaves_of_a_live_graph_of_the_default_stream():
+    x, w = rnd(20, 16, seed=160).requires_grad_(), rnd(16, seed=161).requires_grad_()
+    block = tokens.FeedForwardBlock(16, 40).to(DEV)
+    params = list(block.parameters())
+    h = rnd(20, 16, seed=162, dtype=torch.bfloat16)
+    want = [*torch.autograd.grad(tokens.layer_norm(x, w).sum(), (x, w)), *torch.autograd.grad(block(h).sum(), params)]
+    live = [tokens.layer_norm(x, w), block(h)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="recorded on the default stream"):
+            tokens.layer_norm(x, w)
+        with pytest.raises(RuntimeError, match="recorded on the default stream"):
+            block(h)
+        with torch.no_grad():                                      # (nothing is recorded)
+            unrecorded = tokens.layer_norm(x, w)
+    graph.replay()
+    assert torch.equal(unrecorded, live[0])
+    live.clear()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [*torch.autograd.grad(tokens.layer_norm(x, w).sum(), (x, w)), *torch.autograd.grad(block(h).sum(), params)]
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_opcheck():
