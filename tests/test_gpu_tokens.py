@@ -161,11 +161,11 @@ def test_layer_norm_empty_constant_and_non_finite_rows():
 
 
 # ---- dropout --------------------------------------------------------------------------------------------------------
-def keep_mask(n, p, seed, step, site):
+def keep_mask(n, p, seed, step, site, first=0):
     """Which elements stay, on the CPU, from the generator's definition."""
     m = 0xFFFFFFFF
     c = np.zeros(((n + 7) // 8, 4), np.uint64)
-    c[:, 0] = np.arange(len(c), dtype=np.uint64)
+    c[:, 0] = np.arange(len(c), dtype=np.uint64) + np.uint64(first // 8)
     c[:, 2], c[:, 3] = step & m, site
     k0, k1 = seed & m, (seed >> 32) & m
     for _ in range(7):
@@ -268,7 +268,7 @@ def ternary(rows, cols, seed, dtype):
 
 
 FFN_SHAPES = [(1, 1, 1), (1, 8, 8), (2, 7, 5), (3, 64, 256), (15, 33, 70), (16, 64, 64), (17, 24, 40), (31, 100, 36), (32, 129, 257),
-              (33, 256, 512), (64, 60, 130), (65, 512, 72), (127, 64, 128), (128, 96, 1000), (129, 1000, 96), (257, 180, 360), (300, 136, 264),
+              (33, 256, 512), (40, 1027, 2101), (64, 60, 130), (64, 2048, 1032), (65, 512, 72), (127, 64, 128), (128, 96, 1000), (129, 1000, 96), (257, 180, 360), (300, 136, 264),
               (1000, 65, 129), (2049, 64, 256), (16385, 72, 520), (700, 1024, 2056), (513, 520, 8200)]
 
 
@@ -537,6 +537,68 @@ def test_block_between_convs():
     first, second = run(), run()
     assert all(torch.equal(a, c) for a, c in zip(first, second))
     assert all(g.abs().max() > 0 for g in first)
+
+
+FAR = (1 << 20) + 3                                                # rows of 2056 channels pass 2^31 elements
+
+
+def first_and_last_rows():
+    return torch.cat([torch.arange(40), torch.arange(FAR - 40, FAR)]).to(DEV)
+
+
+def test_gated_ffn_offsets_past_32_bits():
+    """All rows but the first and the last are zeros, which add nothing."""
+    c, f, dtype = 8, 2056, torch.bfloat16
+    at = first_and_last_rows()
+    x, dy = (torch.zeros(FAR, c, dtype=dtype, device=DEV) for _ in range(2))
+    x[at], dy[at] = sparse_ints(80, c, 3, 170, dtype), sparse_ints(80, c, 3, 171, dtype)
+    leaves = [v.requires_grad_() for v in (x, ternary(f, c, 172, dtype), ternary(f, c, 173, dtype), ternary(c, f, 174, dtype))]
+    y = tokens.gated_ffn(*leaves, activation="relu")
+    dx, *dws = torch.autograd.grad(y, leaves, dy)
+    xd, dyd, wg, wu, wd = (v.detach().double() for v in (x[at], dy[at], *leaves[1:]))
+    g, u = xd @ wg.t().contiguous(), xd @ wu.t().contiguous()
+    h = g.clamp_min(0) * u
+    dh = dyd @ wd
+    dg, du = dh * u * (g > 0), dh * g.clamp_min(0)
+    for got, want in zip((y.detach()[at], dx[at], *dws), (h @ wd.t().contiguous(), dg @ wg + du @ wu, dg.t().contiguous() @ xd,
+                                                          du.t().contiguous() @ xd, dyd.t().contiguous() @ h)):
+        assert torch.equal(got, want.to(dtype))
+    assert not y.detach()[40:-40].any() and not dx[40:-40].any()
+
+
+def test_layer_norm_and_dropout_offsets_past_32_bits():
+    c, dtype = 2056, torch.bfloat16
+    at = first_and_last_rows()
+    x = torch.randn(FAR, c, dtype=dtype, device=DEV, generator=torch.Generator(DEV).manual_seed(180)).requires_grad_()
+    w = rnd(c, seed=181).requires_grad_()
+    dy = torch.zeros(FAR, c, dtype=dtype, device=DEV)
+    dy[at] = rnd(80, c, seed=182, dtype=dtype)
+    y = tokens.layer_norm(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    want, tol = norm_bounds(x.detach()[at], w.detach(), None, dy[at], 1e-5, half_step(dtype))
+    for got, k in ((y.detach()[at], 0), (dx[at], 1), (dw, 2)):
+        within(got, want[k], tol[k] + B * want[k].abs() + 1e-30)
+    del y, dx, dy
+    last = FAR * c - 4096
+    x = x.detach()
+    y = tokens.dropout(x, 0.5, state())
+    for first in (0, last):
+        part = x.view(-1)[first:first + 4096]
+        keep = keep_mask(4096, 0.5, -12345678901234567, 3, 0, first)
+        assert torch.equal(y.view(-1)[first:first + 4096], torch.where(keep, part * 2, torch.zeros_like(part)))
+
+
+def test_tied_weights_and_a_skip_from_the_input():
+    """w_gate is w_up and also, transposed by the caller, w_down; dropout's skip is its own input."""
+    x, w, dy = sparse_ints(50, 24, 3, 190, torch.float32), ternary(40, 24, 191, torch.float32), sparse_ints(50, 24, 3, 192, torch.float32)
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    grads = torch.autograd.grad(tokens.gated_ffn(xg, wg, wg, wg.t(), activation="relu"), (xg, wg), dy)
+    apart = [x.clone().requires_grad_(), w.clone().requires_grad_(), w.clone().requires_grad_(), w.t().clone().requires_grad_()]
+    a = torch.autograd.grad(tokens.gated_ffn(*apart, activation="relu"), apart, dy)
+    assert torch.equal(grads[0], a[0]) and torch.equal(grads[1], a[1] + a[2] + a[3].t())
+    xg = x.clone().requires_grad_()
+    (g,) = torch.autograd.grad(tokens.dropout(xg, 0.5, state(), residual=xg), xg, dy)
+    assert torch.equal(g, tokens.dropout(dy, 0.5, state(), residual=dy))
 
 
 def chain(x, ws, rng, dy):
