@@ -6,8 +6,9 @@
 // the gate and the up weights of the same hidden channels, so g and u meet in a wave's registers), one the projection back.
 // Training keeps act(g), u act'(g) and h, inference h alone.  Backward: one launch computes dh and, in its epilogue, dg and
 // du (two products per element: the derivative is taken in the forward pass, from g and u as they were accumulated); one dx,
-// over both sections of k; one all three weight gradients and the bias gradients.  Products accumulate in fp32.  Between the
-// launches h, dg and du are held in the type of x, to which they are rounded as operands of products in any case.
+// over both sections of k; one all three weight gradients and w_down's bias gradient.  Products accumulate in fp32.  Between
+// the launches h, dg and du are held in the type of x, to which they are rounded as operands of products in any case; the other
+// two bias gradients are summed before that rounding, in the epilogue and one more launch.
 //
 // Operands are read 16 bytes at a time.  What does not allow that (a width, stride or pointer that is no multiple of 16
 // bytes) is first copied into padded rows of the workspace, one launch for all of them.
@@ -153,19 +154,19 @@ long long set_tiles(TokGemmArgs &g, bool glu) {
 // last round is (3000 rows, 384 big or 1536 small tiles: 70 against 67; down of 20000 rows, 316 or 1256: 235 against 219).
 bool tiles_are_big(long long big, long long small) { return 1.7 * tok_cdiv(big, N_CU) <= tok_cdiv(small, 2 * N_CU); }
 
-template <typename T, bool A_RC, bool B_RC, int EPI>
+template <typename T, bool A_RC, bool B_RC, int EPI, bool SUMS = false>
 int gemm_pick(TokGemmArgs &g, const char *what, hipStream_t stream) {
     g.splits = 1;
     const bool glu = EPI == TOK_EPI_GLU;
     if constexpr (sizeof(T) == 2) {
         const long long small = set_tiles<Tile128>(g, glu);
-        if (tiles_are_big(set_tiles<Tile256>(g, glu), small)) return gemm_launch<T, Tile256, A_RC, B_RC, EPI>(g, what, stream);
+        if (tiles_are_big(set_tiles<Tile256>(g, glu), small)) return gemm_launch<T, Tile256, A_RC, B_RC, EPI, SUMS>(g, what, stream);
     }
     if (set_tiles<TileSmall<T>>(g, glu) > 0x3fffffffLL) {
         set_error("%s: too many tiles", what);
         return SR355_ERR_INVALID;
     }
-    return gemm_launch<T, TileSmall<T>, A_RC, B_RC, EPI>(g, what, stream);
+    return gemm_launch<T, TileSmall<T>, A_RC, B_RC, EPI, SUMS>(g, what, stream);
 }
 
 // Into how many parts the sum over k of a few tiles is split: the number that takes least, by the rounds of the chip
@@ -356,8 +357,8 @@ struct ForwardPlan : Plan {
     bool split = false;
 };
 
-// The weight gradients, and with them the bias gradients as their left operands' sums: k is the rows.  A bias whose weight
-// needs no gradient takes a product with one column that is not stored.
+// The weight gradients, and with w_down's its bias gradient as the left operand's sums: k is the rows.  Without w_down's, the
+// bias gradient takes a product with one column that is not stored.
 struct WgradShape {
     bool big;
     Splits split;
@@ -365,7 +366,7 @@ struct WgradShape {
 template <typename G>
 long long wgrad_tiles(const sr355_ffn_args *a) {
     auto tiles = [](int M, int N, const void *w, const void *b) { return w || b ? tok_cdiv(M, G::BM) * tok_cdiv(w ? N : 1, G::BN) : 0; };
-    return tiles(a->hidden, a->channels, a->dw_gate_dev, a->db_gate_dev) + tiles(a->hidden, a->channels, a->dw_up_dev, a->db_up_dev) +
+    return tiles(a->hidden, a->channels, a->dw_gate_dev, nullptr) + tiles(a->hidden, a->channels, a->dw_up_dev, nullptr) +
            tiles(a->channels, a->hidden, a->dw_down_dev, a->db_down_dev);
 }
 template <typename G>
@@ -380,12 +381,16 @@ WgradShape wgrad_shape(const sr355_ffn_args *a) {
     return {false, wgrad_splits<Tile128>(a, SmallShape(a->dtype).slots)};
 }
 
+// waves of a tile's rows, each of which leaves column sums of dg and du (of at most as many tiles as small ones are)
+int sum_rows(const sr355_ffn_args *a) { return a->dtype == SR355_DTYPE_F32 ? TileF32::WM : Tile128::WM; }
+static_assert(Tile256::WM == Tile128::WM, "sum_rows");
+
 struct BackwardPlan : Plan {
     Operand x, dy, wg, wu, wd;
     void *dg, *du;
     TokKept kept;
     const void *h;
-    float *parts, *row_parts, *dx_parts;
+    float *parts, *row_parts, *dx_parts, *sums;
     WgradShape wgrad;
     Splits dx;
     bool need_hidden;
@@ -408,12 +413,14 @@ struct BackwardPlan : Plan {
         du = need_hidden ? take(hidden_bytes(a)) : nullptr;
         wgrad = wgrad_shape(a);
         const size_t wide = (size_t)a->hidden * round_up(a->channels, 8), tall = (size_t)a->channels * round_up(a->hidden, 8);
-        const size_t sums = (a->dw_gate_dev ? wide : 0) + (a->dw_up_dev ? wide : 0) + (a->dw_down_dev ? tall : 0);
-        parts = sums && wgrad.split.n > 1 ? (float *)take(wgrad.split.n * sums * sizeof(float)) : nullptr;
+        const size_t weights = (a->dw_gate_dev ? wide : 0) + (a->dw_up_dev ? wide : 0) + (a->dw_down_dev ? tall : 0);
+        parts = weights && wgrad.split.n > 1 ? (float *)take(wgrad.split.n * weights * sizeof(float)) : nullptr;
         dx = {1, 0};
         if (a->dx_dev && a->rows > 0) dx = product_splits(a->rows, a->channels, a->hidden, 2, a->dtype);
         dx_parts = dx.n > 1 ? (float *)take((size_t)dx.n * a->rows * round_up(a->channels, 8) * sizeof(float)) : nullptr;
-        row_parts = wgrad.split.n > 1 ? (float *)take((size_t)wgrad.split.n * (2 * round_up(a->hidden, 8) + round_up(a->channels, 8)) * sizeof(float)) : nullptr;
+        row_parts = wgrad.split.n > 1 && a->db_down_dev ? (float *)take((size_t)wgrad.split.n * round_up(a->channels, 8) * sizeof(float)) : nullptr;
+        sums = a->db_gate_dev || a->db_up_dev
+                   ? (float *)take((size_t)tok_cdiv(a->rows, SmallShape(a->dtype).bm) * sum_rows(a) * 2 * hidden_cols(a) * sizeof(float)) : nullptr;
     }
 };
 
@@ -549,12 +556,12 @@ int ffn_wgrad(const sr355_ffn_args *a, const BackwardPlan &p, hipStream_t stream
             r.job[n_out++] = {j.row_part, sums, 1, M};
         }
     };
-    add(p.dg, hidden_ld(a), p.x.p, p.x.ld, a->hidden, a->channels, a->dw_gate_dev, a->db_gate_dev);
-    add(p.du, hidden_ld(a), p.x.p, p.x.ld, a->hidden, a->channels, a->dw_up_dev, a->db_up_dev);
+    add(p.dg, hidden_ld(a), p.x.p, p.x.ld, a->hidden, a->channels, a->dw_gate_dev, nullptr);
+    add(p.du, hidden_ld(a), p.x.p, p.x.ld, a->hidden, a->channels, a->dw_up_dev, nullptr);
     add(p.dy.p, p.dy.ld, p.h, hidden_ld(a), a->channels, a->hidden, a->dw_down_dev, a->db_down_dev);
     if (!g.n_jobs) return SR355_OK;
     const bool part = g.splits > 1;
-    const bool sums = a->db_gate_dev || a->db_up_dev || a->db_down_dev;
+    const bool sums = a->db_down_dev != nullptr;
     int rc;
     if constexpr (sizeof(T) == 2) {
         if (p.wgrad.big) rc = sums ? wgrad_launch<T, TileWgrad, true>(g, part, stream) : wgrad_launch<T, TileWgrad, false>(g, part, stream);
@@ -572,6 +579,7 @@ int ffn_backward(const sr355_ffn_args *a, hipStream_t stream) {
     BackwardPlan p(a, (unsigned char *)a->workspace_dev);
     int rc = run_pads<T>(p, stream);
     if (rc != SR355_OK) return rc;
+    int n_sums = 0;
     if (p.need_hidden && a->rows > 0) {
         TokGemmArgs g = {};
         g.n_jobs = 1, g.sections = 1, g.act = a->activation, g.K = a->channels;
@@ -580,7 +588,17 @@ int ffn_backward(const sr355_ffn_args *a, hipStream_t stream) {
         j.b[0] = (const unsigned char *)p.wd.p, j.b_ld = p.wd.ld * sizeof(T);
         j.M = (int)a->rows, j.N = a->hidden;
         g.g = p.dg, g.u = p.du, g.kept = p.kept, g.h_ld = hidden_ld(a);
-        rc = gemm_pick<T, false, true, TOK_EPI_GLU_GRAD>(g, "gated_ffn hidden gradient launch", stream);
+        g.sums = p.sums;
+        rc = p.sums ? gemm_pick<T, false, true, TOK_EPI_GLU_GRAD, true>(g, "gated_ffn hidden gradient launch", stream)
+                    : gemm_pick<T, false, true, TOK_EPI_GLU_GRAD>(g, "gated_ffn hidden gradient launch", stream);
+        if (rc != SR355_OK) return rc;
+        n_sums = j.tiles_m * sum_rows(a);
+    }
+    if (p.sums) {
+        const long long first[2] = {0, hidden_cols(a)};
+        const int count[2] = {a->hidden, a->hidden};
+        void *const out[2] = {a->db_gate_dev, a->db_up_dev};
+        rc = launch_tok_sum_parts(p.sums, n_sums, 2 * hidden_cols(a), first, count, out, 2, a->dtype, stream);
         if (rc != SR355_OK) return rc;
     }
     if (a->dx_dev && a->rows > 0) {

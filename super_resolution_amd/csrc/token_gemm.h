@@ -69,6 +69,7 @@ struct TokGemmArgs {
     const void *bias_up;                // GLU
     TokKept kept;                       // GLU: written where not null; gradient: read
     void *g, *u, *h;                    // GLU: the product (h); gradient: dg, du
+    float *sums;                        // gradient: [tiles_m * WM][dg, du][N rounded up to 8], column sums of a wave's rows
     long long h_ld;                     // elements, of g / u / h / dg / du; a multiple of 16 bytes
 };
 
@@ -394,14 +395,19 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
     // fragments of two k steps: the one being multiplied and the next
-    // Sums of A over k (the bias gradients, for which A would be read again): the waves of the first column of tiles that hold
-    // its first columns add up the fragments as they pass, one lane per row and half of k.  A variant of its own: the branch
-    // in the main loop costs 7 % where nothing is summed.
-    static_assert(!SUMS || (A_RC && (EPI == TOK_EPI_STORE || EPI == TOK_EPI_PART)), "sums of a left operand strided in k");
-    const bool sums = SUMS && tn == 0 && wn == 0 && job.row_sums;
-    float row_sum[SUMS ? MT : 1];
+    // SUMS, a weight gradient: sums of A over k (a bias gradient, for which A would be read again): the waves of the first
+    // column of tiles that hold its first columns add up the fragments as they pass, one lane per row and half of k.  A variant
+    // of its own: the branch in the main loop costs 7 % where nothing is summed.
+    // SUMS, the hidden gradient: sums of dg and du over a wave's rows, before they are rounded.
+    static_assert(!SUMS || EPI == TOK_EPI_GLU_GRAD || (A_RC && (EPI == TOK_EPI_STORE || EPI == TOK_EPI_PART)), "what is summed");
+    constexpr bool ROW_SUMS = SUMS && EPI != TOK_EPI_GLU_GRAD, COL_SUMS = SUMS && EPI == TOK_EPI_GLU_GRAD;
+    const bool sums = ROW_SUMS && tn == 0 && wn == 0 && job.row_sums;
+    float row_sum[ROW_SUMS ? MT : 1];
 #pragma unroll
-    for (int i = 0; i < (SUMS ? MT : 1); ++i) row_sum[i] = 0.f;
+    for (int i = 0; i < (ROW_SUMS ? MT : 1); ++i) row_sum[i] = 0.f;
+    float col_sum[COL_SUMS ? 16 : 1];                      // dg's of this lane's eight columns, then du's
+#pragma unroll
+    for (int i = 0; i < (COL_SUMS ? 16 : 1); ++i) col_sum[i] = 0.f;
     auto add_sums = [&](const tok_v4u (&a)[MT]) {
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
@@ -503,7 +509,7 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
                 __builtin_amdgcn_s_barrier();
                 asm volatile("" ::: "memory");
             }
-            if constexpr (SUMS) {
+            if constexpr (ROW_SUMS) {
                 if (sums) add_sums(f.a);
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -546,7 +552,7 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
     // and its fetch took longer than the main loop (training step of 16384 x 1024 x 4096: 354 + 310 us for the two products
     // with an activation).
     constexpr bool EXACT = sizeof(T) == 4;
-    if constexpr (SUMS) {
+    if constexpr (ROW_SUMS) {
         if (sums) {
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
@@ -609,6 +615,10 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
                     float dg[8], du[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) dg[j] = v[j] * kd[k].value(j), du[j] = v[j] * ka[k].value(j);
+                    if constexpr (COL_SUMS) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) col_sum[j] += dg[j], col_sum[8 + j] += du[j];
+                    }
                     tok_store8<T>((T *)p.g + m * p.h_ld + n, dg);
                     tok_store8<T>((T *)p.u + m * p.h_ld + n, du);
                 }
@@ -686,6 +696,18 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
         } else {
             if (wide) finish(std::integral_constant<int, WIDE>{}, m_first);
             else finish(std::integral_constant<int, NARROW>{}, m_first);
+        }
+    }
+    if constexpr (COL_SUMS) {
+        // the lanes that hold the same columns, in a fixed order
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+#pragma unroll
+            for (int o = LANES; o < 64; o <<= 1) col_sum[j] += __shfl_xor(col_sum[j], o, 64);
+        if (lane < LANES && in_n) {
+            float *part = p.sums + ((size_t)tm * G::WM + wm) * 2 * n_stored + n;
+            tok_store8<float>(part, *reinterpret_cast<const float(*)[8]>(col_sum));
+            tok_store8<float>(part + n_stored, *reinterpret_cast<const float(*)[8]>(col_sum + 8));
         }
     }
 }
