@@ -160,9 +160,10 @@ class Sr355Error(RuntimeError):
     pass
 
 
-def build(verbose: bool = False) -> str:
-    """Compile libsr355.so for gfx950 with hipcc (works without a GPU)."""
-    cmd = ["make", "-C", CSRC_DIR, "-j8"]
+def build(verbose: bool = False, again: bool = False) -> str:
+    """Compile libsr355.so for gfx950 with hipcc, and the binding beside it (works without a GPU); ``again``: also what is up
+    to date."""
+    cmd = ["make", "-C", CSRC_DIR, "-j8", *(["-B"] if again else [])]
     res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if verbose or res.returncode:
         print(res.stdout)

@@ -101,7 +101,7 @@ class FeedForwardBlock(nn.Module):
         if x.dim() < 1 or x.shape[-1] != self.channels:
             raise RuntimeError(f"FeedForwardBlock: expected rows of {self.channels} channels, got {tuple(x.shape)}")
 
-        if torch.is_grad_enabled() and x.is_cuda:
+        if torch.is_grad_enabled() and x.is_cuda and torch.cuda.is_current_stream_capturing():
             ops.binding().check_capture([x, *self.parameters()])     # (the calls see the parameters' copies in x's type)
 
         def typed(t: Optional[Tensor]) -> Optional[Tensor]:
