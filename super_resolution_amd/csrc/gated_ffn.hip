@@ -25,6 +25,9 @@ namespace {
 typedef TokTile<256, 256, 2, 4, 128, 2> Tile256;
 typedef TokTile<256, 256, 2, 4, 64, 5> TileWgrad;
 typedef TokTile<128, 128, 2, 2, 128, 2> Tile128;
+// As many small tiles as CUs or fewer: one per CU, so the ring may take three stages (bf16, gate / up of 65 rows, 2048 x 8192:
+// 22 against 27 us, 1024 x 4096: 15 against 17, of 200 rows 26 against 30; four stages take no less).
+typedef TokTile<128, 128, 2, 2, 128, 3> TileFew;
 constexpr int N_CU = 256;
 
 // fp32: 32 x 32 x 2 instructions take eight times as long for the same bytes, so operand traffic does not matter and small tiles,
@@ -160,6 +163,7 @@ int gemm_pick(TokGemmArgs &g, const char *what, hipStream_t stream) {
     const bool glu = EPI == TOK_EPI_GLU;
     if constexpr (sizeof(T) == 2) {
         const long long small = set_tiles<Tile128>(g, glu);
+        if (small <= N_CU) return gemm_launch<T, TileFew, A_RC, B_RC, EPI, SUMS>(g, what, stream);
         if (tiles_are_big(set_tiles<Tile256>(g, glu), small)) return gemm_launch<T, Tile256, A_RC, B_RC, EPI, SUMS>(g, what, stream);
     }
     if (set_tiles<TileSmall<T>>(g, glu) > 0x3fffffffLL) {
@@ -297,8 +301,20 @@ bool narrow_fits(const sr355_ffn_args *a) {
     return !a->saved_dev && a->dtype != SR355_DTYPE_F32 && a->channels <= 128 && a->rows >= 64LL * N_CU;
 }
 
-// up to so many rows the kernels of token_rows.h: reading the weights bounds them
+// Few rows, the kernels of token_rows.h: reading the weights bounds them.  Their workgroups each read all rows, 16 or fewer
+// channels' worth, so with many rows and channels the tiles of 128 rows are faster, split over k for down (bf16, us:
+//     rows                 16        32        64
+//     gate / up 1024 x 4096    6 / 15    7 / 15   11 / 15
+//               2048 x 8192   15 / 22   18 / 22   27 / 22
+//     down      1024 x 4096    8 / 10   12 / 10   19 / 12
+//               2048 x 8192   14 / 15   22 / 15   37 / 17, rows / tiles).  fp32 tiles are bound by the matrix pipes even then.
 constexpr int FEW_ROWS = 64;
+bool few_glu(const sr355_ffn_args *a) {
+    return a->rows <= 32 || (a->rows <= FEW_ROWS && (a->dtype == SR355_DTYPE_F32 || (long long)a->channels * a->hidden <= (1 << 23)));
+}
+bool few_down(const sr355_ffn_args *a) {
+    return a->rows <= 16 || (a->rows <= FEW_ROWS && (a->dtype == SR355_DTYPE_F32 || (long long)a->channels * a->hidden <= (1 << 21)));
+}
 
 // a call's saved buffer: h, the two kept arrays, their low parts
 struct Saved {
@@ -316,13 +332,6 @@ struct Saved {
         kept.a_low = (unsigned char *)take((size_t)a->rows * hidden_ld(a)), kept.d_low = (unsigned char *)take((size_t)a->rows * hidden_ld(a));
     }
 };
-
-// Down of few rows: that kernel's workgroups each read all rows, 16 or fewer channels' worth, so with many rows and channels
-// the split product of 128-row tiles is faster (bf16, 2048 x 8192: 16 rows 14 against 15 us, 32 rows 22 against 15, 64 rows 37
-// against 17; 1024 x 4096: 8, 12 and 19 against 10, 10 and 12).  fp32 tiles are bound by the matrix pipes even then.
-bool few_down(const sr355_ffn_args *a) {
-    return a->rows <= 16 || (a->rows <= FEW_ROWS && (a->dtype == SR355_DTYPE_F32 || (long long)a->channels * a->hidden <= (1 << 21)));
-}
 
 struct ForwardPlan : Plan {
     Operand x, wg, wu, wd;
@@ -514,7 +523,7 @@ int ffn_forward(const sr355_ffn_args *a, hipStream_t stream) {
     j.b[0] = (const unsigned char *)p.wg.p, j.b[1] = (const unsigned char *)p.wu.p, j.b_ld = p.wg.ld * sizeof(T);
     j.M = (int)a->rows, j.N = a->hidden, j.bias = a->b_gate_dev;
     g.bias_up = a->b_up_dev, g.kept = p.kept, g.h = p.h, g.h_ld = hidden_ld(a);
-    rc = a->rows <= FEW_ROWS ? ffn_glu_few<T>(a, p, stream) : gemm_pick<T, false, false, TOK_EPI_GLU>(g, "gated_ffn gate / up launch", stream);
+    rc = few_glu(a) ? ffn_glu_few<T>(a, p, stream) : gemm_pick<T, false, false, TOK_EPI_GLU>(g, "gated_ffn gate / up launch", stream);
     if (rc != SR355_OK) return rc;
     if (few_down(a)) return ffn_down_few<T>(a, p, stream);
     TokGemmArgs d = {};

@@ -4,7 +4,7 @@
 // MFMA (weights as its rows, the tensor's rows as its columns, 16 at a time), and add up in the LDS in wave order.  A wave
 // instruction reads 64 consecutive bytes of 16 rows.
 // Measured (bf16): 1 row, 1024 x 4096: 5.0 + 5.1 us (16.8 and 8.4 MB of weights, the launch is half of it); 27 rows,
-// 2048 x 8192: 17 us for the 67 MB of gate and up (3.9 TB/s; the tiles of 128 rows 25).  Its down product would take 20 us for
+// 2048 x 8192: 17 us for the 67 MB of gate and up (3.9 TB/s; the tiles of 128 rows 21).  Its down product would take 20 us for
 // 33 MB, since each of 256 workgroups also reads all 442 KB of rows from the L2 (4 channels a workgroup, which read the rows
 // more often, 35; 16, which leave CUs idle, 22): with so many rows the split product takes it, in 15.
 #pragma once
