@@ -20,6 +20,8 @@ struct TokRowsArgs {
     int channels;                         // output channels of a workgroup: 16, or fewer where that leaves CUs idle
     const void *bias, *bias2;
     void *out;                            // GLU: h
+    const unsigned char *x_low;           // LOW: what h's rounding to the type left, added to the product
+    void *out_low;                        // GLU: written where not null
     TokKept kept;                         // GLU: written where not null
     long long out_ld;                     // elements
     int n_store;                          // columns stored (GLU: up to the next eighth)
@@ -39,11 +41,12 @@ __device__ __forceinline__ void tok_mfma16(const tok_v4u &a, const tok_v4u &b, t
     }
 }
 
-// TG groups of 16 rows; GLU: two weights and the activation, else one weight.
-template <typename T, int TG, bool GLU, int WAVES>
+// TG groups of 16 rows; GLU: two weights and the activation, else one weight.  LOW: the rows are the sum of two arrays, both
+// multiplied with the weights as they pass: h keeps twice its bits in small blocks.
+template <typename T, int TG, bool GLU, int WAVES, bool LOW>
 __device__ __forceinline__ void tok_rows_body(const TokRowsArgs &p) {
     constexpr unsigned OUT = 0x80000000u;
-    constexpr int Q = GLU ? 2 : 1;
+    constexpr int Q = GLU ? 2 : 1, P = LOW ? 2 : 1;
     __shared__ float red[WAVES][Q * TG][16][17];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int i = lane & 15, g = lane >> 4;
@@ -53,6 +56,8 @@ __device__ __forceinline__ void tok_rows_body(const TokRowsArgs &p) {
     const __amdgpu_buffer_rsrc_t rw2 =
         __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char *>((GLU ? p.w2 : p.w) + n0 * p.w_ld), 0, 0x7fffffff, 0x00020000);
     const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char *>(p.x), 0, 0x7fffffff, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rl =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char *>(LOW ? p.x_low : p.x), 0, 0x7fffffff, 0x00020000);
     const unsigned vw = i < p.channels && n0 + i < p.N ? (unsigned)(i * p.w_ld + g * 16) : OUT;
     unsigned vx[TG];
 #pragma unroll
@@ -69,7 +74,7 @@ __device__ __forceinline__ void tok_rows_body(const TokRowsArgs &p) {
     // UN blocks' reads in flight (four take no less time); a block past the end reads zeros
     constexpr int UN = 2;
     for (int b = wave; b < blocks; b += WAVES * UN) {
-        tok_v4u w[UN][Q][2], x[UN][TG][2];
+        tok_v4u w[UN][Q][2], x[UN][P * TG][2];
 #pragma unroll
         for (int k = 0; k < UN; ++k) {
             const int turn = b + k * WAVES, block = turn + first;
@@ -81,7 +86,10 @@ __device__ __forceinline__ void tok_rows_body(const TokRowsArgs &p) {
                 w[k][0][u] = __builtin_amdgcn_raw_buffer_load_b128(rw, in ? vw + at + u * 64 : OUT, 0, 0);
                 if constexpr (GLU) w[k][Q - 1][u] = __builtin_amdgcn_raw_buffer_load_b128(rw2, in ? vw + at + u * 64 : OUT, 0, 0);
 #pragma unroll
-                for (int t = 0; t < TG; ++t) x[k][t][u] = __builtin_amdgcn_raw_buffer_load_b128(rx, in ? vx[t] + at + u * 64 : OUT, 0, 0);
+                for (int t = 0; t < TG; ++t) {
+                    x[k][t][u] = __builtin_amdgcn_raw_buffer_load_b128(rx, in ? vx[t] + at + u * 64 : OUT, 0, 0);
+                    if constexpr (LOW) x[k][TG + t][u] = __builtin_amdgcn_raw_buffer_load_b128(rl, in ? vx[t] + at + u * 64 : OUT, 0, 0);
+                }
             }
         }
         __builtin_amdgcn_sched_barrier(0);                  // (all of them go out before the first is waited for)
@@ -92,7 +100,10 @@ __device__ __forceinline__ void tok_rows_body(const TokRowsArgs &p) {
 #pragma unroll
                 for (int t = 0; t < TG; ++t)
 #pragma unroll
-                    for (int q = 0; q < Q; ++q) tok_mfma16<T>(w[k][q][u], x[k][t][u], acc[q][t]);
+                    for (int q = 0; q < Q; ++q) {
+                        tok_mfma16<T>(w[k][q][u], x[k][t][u], acc[q][t]);
+                        if constexpr (LOW) tok_mfma16<T>(w[k][q][u], x[k][(P - 1) * TG + t][u], acc[q][t]);
+                    }
     }
     // accumulator element e: n = 4 * (lane >> 4) + e, row = lane & 15
 #pragma unroll
@@ -122,7 +133,10 @@ __device__ __forceinline__ void tok_rows_body(const TokRowsArgs &p) {
             else if (p.act == SR355_ACT_GELU) tok_act_grad<EXACT, SR355_ACT_GELU>(v[0], a, d);
             else if (p.act == SR355_ACT_RELU) tok_act_grad<EXACT, SR355_ACT_RELU>(v[0], a, d);
             else tok_act_grad<EXACT, SR355_ACT_SIGMOID>(v[0], a, d);
-            ((T *)p.out)[at] = (T)(a * v[Q - 1]);
+            const float h = a * v[Q - 1];
+            const T high = (T)h;
+            ((T *)p.out)[at] = high;
+            if (p.out_low) ((T *)p.out_low)[at] = (T)(__builtin_isfinite((float)high) ? h - (float)high : 0.f);
             if (p.kept.a) {
                 tok_keep<T>(p.kept.a, p.kept.a_low, at, a);
                 tok_keep<T>(p.kept.d, p.kept.d_low, at, v[Q - 1] * d);
@@ -133,9 +147,9 @@ __device__ __forceinline__ void tok_rows_body(const TokRowsArgs &p) {
     }
 }
 
-template <typename T, int TG, bool GLU, int WAVES>
+template <typename T, int TG, bool GLU, int WAVES, bool LOW>
 __global__ __launch_bounds__(64 * WAVES) void tok_rows_kernel(TokRowsArgs p) {
-    tok_rows_body<T, TG, GLU, WAVES>(p);
+    tok_rows_body<T, TG, GLU, WAVES, LOW>(p);
 }
 
 }  // namespace

@@ -333,8 +333,10 @@ def test_gated_ffn_unrecorded_on_many_narrow_rows_matches_the_formula(act, dtype
         assert y[7].isnan().all() and y[:7].isfinite().all() and y[8:].isfinite().all()
 
 
-def ffn_bounds(x, dy, ws, bs, act, u):
-    """Results and bounds in 64 bits.  Per sum of n products: n B of the sum of magnitudes; u per rounding to the type."""
+def ffn_bounds(x, dy, ws, bs, act, u, uh=None):
+    """Results and bounds in 64 bits.  Per sum of n products: n B of the sum of magnitudes; u per rounding to the type (uh: of
+    h, dg and du, where that is another)."""
+    uh = u if uh is None else uh
     t, c = x.shape
     f = ws[0].shape[0]
     xd, dyd = x.double(), dy.double()
@@ -353,7 +355,7 @@ def ffn_bounds(x, dy, ws, bs, act, u):
     e_u = (c + 4) * B * (xd.abs() @ T(wu.abs()) + bu.abs()) + 4 * B * uu.abs()
     fn = 2.0 ** -20                                            # the activations' own error, relative to max(|a|, |a'|)
     e_a = 1.13 * e_g + fn * a.abs()
-    e_h = e_a * uu.abs() + a.abs() * e_u + 2 * u * h.abs()
+    e_h = e_a * uu.abs() + a.abs() * e_u + 2 * uh * h.abs()
     y = h @ T(wd) + bd
     t_y = e_h @ T(wd.abs()) + (f + 4) * B * (h.abs() @ T(wd.abs()) + bd.abs()) + u * y.abs()
     # the backward pass multiplies dh with act(g) and u act'(g), kept as the upper 24 bits of fp32 (cut: off by less than
@@ -366,8 +368,8 @@ def ffn_bounds(x, dy, ws, bs, act, u):
     e_as = e_a + 1.01 * cut * a.abs()
     e_d = e_u * (da.abs() + e_da) + uu.abs() * e_da + 1.01 * cut * (uu * da).abs() + 4 * B * (uu * da).abs()
     grow = 1.01
-    e_dg = grow * (e_dh * (uu * da).abs() + dh.abs() * e_d + 4 * B * dg.abs()) + 1.01 * u * dg.abs()
-    e_du = grow * (e_dh * a.abs() + dh.abs() * e_as + 4 * B * du.abs()) + 1.01 * u * du.abs()
+    e_dg = grow * (e_dh * (uu * da).abs() + dh.abs() * e_d + 4 * B * dg.abs()) + 1.01 * uh * dg.abs()
+    e_du = grow * (e_dh * a.abs() + dh.abs() * e_as + 4 * B * du.abs()) + 1.01 * uh * du.abs()
     dx = dg @ wg + du @ wu
     t_dx = e_dg @ wg.abs() + e_du @ wu.abs() + (2 * f + 4) * B * (dg.abs() @ wg.abs() + du.abs() @ wu.abs()) + u * dx.abs()
     out, tol = [y, dx], [t_y, t_dx]
@@ -397,6 +399,32 @@ def test_gated_ffn_matches_the_formula(shape, act, dtype):
         tiny = torch.finfo(dtype).tiny * (1 + f)
         for name, a, b, e in zip(("y", "dx", "dw_gate", "dw_up", "dw_down", "db_gate", "db_up", "db_down"), (y, *grads), want, tol):
             within(a, b, e + tiny, name)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1, 20, 1700), (5, 33, 96), (16, 40, 640), (20, 24, 500), (61, 16, 520)])
+def test_gated_ffn_of_a_small_block_rounds_once(shape, dtype):
+    """Few rows of few channels: h is a sum of two numbers of the type, whose rounding is u^2 (fp16: half a smallest subnormal at least,
+    2^-25).  Bias gradients of gate and up, of any rows: dg and du are summed in fp32."""
+    t, c, f = shape
+    x, dy, ws, bs = ffn_inputs(t, c, f, dtype, True, 40)
+    leaves = [v.clone().requires_grad_() for v in (x, *ws, *bs)]
+    y = tokens.gated_ffn(*leaves)
+    grads = torch.autograd.grad(y, leaves, dy)
+    u = half_step(dtype)
+    want, tol = ffn_bounds(x, dy, ws, bs, "silu", u, 1.01 * u * u)
+    low = 2.0 ** -25 if dtype == torch.float16 else 1e-30
+    tiny = torch.finfo(dtype).tiny
+    within(y, want[0], tol[0] + low * ws[2].double().abs().sum(1) + tiny, "y")
+    within(tokens.gated_ffn(x, *ws, *bs), want[0], tol[0] + low * ws[2].double().abs().sum(1) + tiny, "y unrecorded")
+    for k in (5, 6):
+        within(grads[k - 1], want[k], tol[k] + tiny * (1 + t), k)
+    x[0, 0] = float("inf")
+    assert tokens.gated_ffn(x, *ws, *bs)[0].isnan().any() and tokens.gated_ffn(x, *ws, *bs)[1:].isfinite().all()
+    huge = torch.full((1, c), 200.0, dtype=dtype, device=DEV)       # h is infinite in fp16, and so is y, without a NaN
+    ones = [torch.ones_like(w) for w in ws]
+    out = tokens.gated_ffn(huge, *ones, activation="relu")
+    assert not out.isnan().any() and (out.isinf().all() if dtype == torch.float16 else out.isfinite().all())
 
 
 def test_gated_ffn_gradients_against_differences():
