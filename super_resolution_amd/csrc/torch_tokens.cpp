@@ -353,6 +353,7 @@ variable_list gated_ffn_bwd(const Tensor &dy, const Tensor &x, const Tensor &w_g
     check_device(who, x, saved);
     TORCH_CHECK(dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type() && need.size() == 7,
                 who, ": the gradient must have x's shape and type");
+    TORCH_CHECK(saved.scalar_type() == at::kByte && saved.is_contiguous(), who, ": what the forward pass saved is a contiguous tensor of bytes");
     const Rows g(dy);
     a.dy_dev = g.data(), a.dy_ld = g.ld;
     a.saved_dev = a.rows ? const_cast<void *>(saved.const_data_ptr()) : nullptr, a.saved_bytes = static_cast<size_t>(saved.numel());

@@ -762,6 +762,10 @@ def test_refusals():
         with pytest.raises(RuntimeError, match=match):
             call()
             pytest.fail(f"call {k} was not refused")
+    saved = token_ops.gated_ffn_fwd(x, w, w, wd, None, None, None, 0, True)[1]
+    for s in (saved[:1].expand(saved.numel()), saved.float(), saved[:-512], saved[8:]):
+        with pytest.raises(RuntimeError, match="saved"):
+            token_ops.gated_ffn_bwd(x, x, w, w, wd, s, 0, [True] * 7)
     # gradients are once differentiable, and say so
     xg = x.clone().requires_grad_()
     (g,) = torch.autograd.grad(tokens.layer_norm(xg).square().sum(), xg, create_graph=True)
