@@ -260,15 +260,31 @@ struct Plan {
         at += (bytes + 255) & ~(size_t)255;
         return r;
     }
-    // the operand as it is where 16-byte reads can have it, else its padded copy
-    Operand operand(const void *p, long long rows, int cols, long long ld, int dtype) {
+    // whether 16-byte reads can have the operand as it is
+    static bool in_place(const void *p, int cols, long long ld, int dtype) {
         const int e = dtype == SR355_DTYPE_F32 ? 4 : 8;
-        const long long row_bytes = ld * (long long)tok_type_bytes(dtype);
-        if (cols % e == 0 && ld % e == 0 && tok_aligned16(p) && row_bytes < (1LL << 22)) return {p, ld};
+        return cols % e == 0 && ld % e == 0 && tok_aligned16(p) && ld * (long long)tok_type_bytes(dtype) < (1LL << 22);
+    }
+    Operand copy(const void *p, long long rows, int cols, long long ld, int dtype) {
         const long long dst_ld = row_ld(cols, dtype);
         void *dst = take((size_t)rows * dst_ld * tok_type_bytes(dtype));
         pads.job[n_pads++] = {p, dst, rows, ld, dst_ld, cols};
         return {dst, dst_ld};
+    }
+    // the operand as it is where that can be, else its padded copy
+    Operand operand(const void *p, long long rows, int cols, long long ld, int dtype) {
+        return in_place(p, cols, ld, dtype) ? Operand{p, ld} : copy(p, rows, cols, ld, dtype);
+    }
+    // The gate and up weights, which the kernels read with one row stride: both as they are, or copies of both (a copy's rows
+    // may be longer than the weight's, see row_ld).
+    void gate_and_up(const sr355_ffn_args *a, Operand &wg, Operand &wu) {
+        const int c = a->channels;
+        if (in_place(a->w_gate_dev, c, c, a->dtype) && in_place(a->w_up_dev, c, c, a->dtype)) {
+            wg = {a->w_gate_dev, c}, wu = {a->w_up_dev, c};
+        } else {
+            wg = copy(a->w_gate_dev, a->hidden, c, c, a->dtype);
+            wu = copy(a->w_up_dev, a->hidden, c, c, a->dtype);
+        }
     }
 };
 
@@ -350,8 +366,7 @@ struct ForwardPlan : Plan {
     ForwardPlan(const sr355_ffn_args *a, unsigned char *ws) {
         base = ws;
         x = operand(a->x_dev, a->rows, a->channels, a->x_ld, a->dtype);
-        wg = operand(a->w_gate_dev, a->hidden, a->channels, a->channels, a->dtype);
-        wu = operand(a->w_up_dev, a->hidden, a->channels, a->channels, a->dtype);
+        gate_and_up(a, wg, wu);
         wd = operand(a->w_down_dev, a->channels, a->hidden, a->hidden, a->dtype);
         if (a->saved_dev) {
             const Saved s(a, (unsigned char *)a->saved_dev);
@@ -418,10 +433,7 @@ struct BackwardPlan : Plan {
         x = wg = wu = wd = {nullptr, 0};
         dy = operand(a->dy_dev, a->rows, a->channels, a->dy_ld, a->dtype);
         if (gate_up) x = operand(a->x_dev, a->rows, a->channels, a->x_ld, a->dtype);
-        if (a->dx_dev) {
-            wg = operand(a->w_gate_dev, a->hidden, a->channels, a->channels, a->dtype);
-            wu = operand(a->w_up_dev, a->hidden, a->channels, a->channels, a->dtype);
-        }
+        if (a->dx_dev) gate_and_up(a, wg, wu);
         if (need_hidden) wd = operand(a->w_down_dev, a->channels, a->hidden, a->hidden, a->dtype);
         const Saved s(a, (unsigned char *)a->saved_dev);
         kept = s.kept, h = s.h;

@@ -1,0 +1,57 @@
+"""GPU: the operators on rows of channels where one argument differs from what the others are like, and on rows and values at
+the ends of their ranges.  Products of small integers are exact, so results have to be equal."""
+import pytest
+import torch
+
+from super_resolution_amd import tokens
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def rnd(*shape, seed=0, scale=1.0, shift=0.0, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * scale + shift).to(dtype).to(DEV)
+
+
+def sparse_ints(rows, cols, per_row, seed, dtype):
+    g = torch.Generator().manual_seed(seed)
+    at = torch.randint(0, cols, (rows, per_row), generator=g)
+    return torch.zeros(rows, cols).scatter_(1, at, torch.randint(0, 2, (rows, per_row), generator=g) * 2.0 - 1).to(dtype).to(DEV)
+
+
+def ternary(rows, cols, seed, dtype):
+    return torch.randint(-1, 2, (rows, cols), generator=torch.Generator().manual_seed(seed)).to(dtype).to(DEV)
+
+
+def T(m):
+    return m.t().contiguous()
+
+
+def relu_block(x, dy, wg, wu, wd):
+    """y and the gradients of x and the weights in 64 bits."""
+    x, dy, wg, wu, wd = (v.double() for v in (x, dy, wg, wu, wd))
+    g, u = x @ T(wg), x @ T(wu)
+    h, dh = g.clamp_min(0) * u, dy @ wd
+    dg, du = dh * u * (g > 0), dh * g.clamp_min(0)
+    return h @ T(wd), dg @ wg + du @ wu, T(dg) @ x, T(du) @ x, T(dy) @ h
+
+
+@pytest.mark.parametrize("dtype,c", [(torch.bfloat16, 264), (torch.float16, 1000), (torch.float32, 20), (torch.float32, 132)])
+@pytest.mark.parametrize("rows", [1, 33, 70, 300])
+def test_one_weight_at_an_odd_address(rows, c, dtype):
+    """As a view into one flat buffer of parameters has it.  |g|, |u| <= 3, |dh| <= 3: every intermediate is exact in every type."""
+    f = 56
+    x, dy = sparse_ints(rows, c, 3, 1, dtype), sparse_ints(rows, c, 3, 2, dtype)
+    ws = [ternary(f, c, 3, dtype), ternary(f, c, 4, dtype), ternary(c, f, 5, dtype)]
+    want = [v.to(dtype) for v in relu_block(x, dy, *ws)]
+    for moved in range(3):
+        args = list(ws)
+        args[moved] = torch.empty(ws[moved].numel() + 1, dtype=dtype, device=DEV)[1:].view(ws[moved].shape).copy_(ws[moved])
+        leaves = [v.detach().requires_grad_() for v in (x, *args)]
+        y = tokens.gated_ffn(*leaves, activation="relu")
+        for got, w in zip((y, *torch.autograd.grad(y, leaves, dy)), want):
+            assert torch.equal(got, w), moved
+        with torch.no_grad():
+            assert torch.equal(tokens.gated_ffn(x, *args, activation="relu"), y), moved

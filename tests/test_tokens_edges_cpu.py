@@ -1,0 +1,42 @@
+"""CPU: the operators on rows of channels where a call's arguments, not its numbers, decide what happens.  No kernel runs
+here."""
+import ctypes as C
+
+import pytest
+
+from super_resolution_amd import _lib
+from super_resolution_amd._lib import FfnArgs
+
+
+@pytest.fixture(scope="module")
+def L():
+    return _lib.lib()
+
+
+P = 4096   # an address that nothing reads
+
+
+def ffn(**kw):
+    a = FfnArgs()
+    a.rows, a.channels, a.hidden = 70, 264, 520
+    for k, v in kw.items():
+        setattr(a, k, v)
+    a.x_ld = a.dy_ld = a.channels
+    for k in ("x_dev", "w_gate_dev", "w_up_dev", "w_down_dev", "y_dev", "dy_dev", "dx_dev", "workspace_dev", "saved_dev"):
+        if not getattr(a, k):
+            setattr(a, k, P)
+    return C.byref(a)
+
+
+@pytest.mark.parametrize("dtype,channels", [(_lib.DTYPE_BF16, 264), (_lib.DTYPE_F16, 1000), (_lib.DTYPE_BF16, 2056), (_lib.DTYPE_F32, 20),
+                                            (_lib.DTYPE_F32, 100), (_lib.DTYPE_F32, 132)])
+@pytest.mark.parametrize("rows", [1, 33, 70, 300])
+@pytest.mark.parametrize("backward", [0, 1])
+def test_gate_and_up_weights_are_padded_together(L, dtype, channels, rows, backward):
+    """The kernels read both with one row stride, and a padded copy's rows are longer at these widths: where one of the two has to
+    be copied, both are."""
+    size = lambda **kw: L.sr355_gated_ffn_workspace_bytes(ffn(dtype=dtype, channels=channels, rows=rows, **kw), backward)
+    odd = P + 4
+    both = size(w_gate_dev=odd, w_up_dev=odd)
+    assert both > size()
+    assert size(w_gate_dev=odd) == both and size(w_up_dev=odd) == both
