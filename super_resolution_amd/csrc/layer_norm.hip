@@ -3,9 +3,12 @@
 //     dw = sum over rows of dy * xh, db = sum over rows of dy.
 // Both directions are bound by memory: forward reads x and writes y, backward reads x and dy and writes dx.  A row is
 // held in registers by L lanes (8 to 64 of a wave, or a workgroup of 256), so it is read once and the variance is the
-// mean of squared deviations from the mean (E[x^2] - mean^2 loses it where the mean dominates).  Statistics, sums and
-// the two row means are fp32.  The backward pass keeps dw / db of the lane's columns in registers over all rows of the
-// workgroup and writes one partial row per workgroup; a second launch adds the partials in order.  No atomics.
+// mean of squared deviations from the mean (E[x^2] - mean^2 loses it where the mean dominates).  The forward pass takes the
+// channels' distances from the row's first one before it sums: what is common to them costs no bits, and equal channels are
+// zeros (as sums of x, times the rounded 1 / C, 999 channels of 1000.1 gave a mean one step off and y = 0.04; it takes 1.4 us
+// of 32768 x 1024 bf16's 26).  The backward pass takes the mean as it is stored, rounded to fp32.  Statistics, sums and the two
+// row means are fp32.  The backward pass keeps dw / db of the lane's columns in registers over all rows of the workgroup and
+// writes one partial row per workgroup; a second launch adds the partials in order.  No atomics.
 #include "token_common.h"
 
 namespace sr355 {
@@ -55,6 +58,9 @@ struct LnArgs {
     float eps;
 };
 
+// What a row's channels are measured from: its first one, unless that is so large that a difference could overflow (or no number).
+__device__ __forceinline__ float ln_origin(float first) { return fabsf(first) < 0x1p100f ? first : 0.f; }
+
 // The row in registers: lane l of L holds units l, l + L, ... of E elements.
 template <typename T, int E, int L, int U>
 __global__ __launch_bounds__(LN_THREADS) void ln_fwd_kernel(LnArgs a) {
@@ -66,30 +72,42 @@ __global__ __launch_bounds__(LN_THREADS) void ln_fwd_kernel(LnArgs a) {
     for (long long row = (long long)blockIdx.x * ROWS + threadIdx.x / L; row < a.rows; row += (long long)gridDim.x * ROWS) {
         const T *x = (const T *)a.x + row * a.x_ld;
         float v[U][E];
-        float s = 0.f;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int c = (u * L + l) * E;
 #pragma unroll
             for (int j = 0; j < E; ++j) v[u][j] = 0.f;
             if (c < a.C) tok_load<T, E>(x + c, v[u]);
+        }
+        float first;                                        // (the row's first lane has its first channel)
+        if constexpr (L < 64) first = __shfl(v[0][0], 0, L);
+        else if constexpr (L == 64) first = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v[0][0])));
+        else first = (float)x[0];
+        const float origin = ln_origin(first);
+        float s = 0.f;
 #pragma unroll
-            for (int j = 0; j < E; ++j) s += v[u][j];
+        for (int u = 0; u < U; ++u) {
+            if ((u * L + l) * E >= a.C) continue;
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                v[u][j] -= origin;
+                s += v[u][j];
+            }
         }
         const float mean = row_sum<L>(s, red, turn) * inv_c;
+        if (l == 0 && a.mean) a.mean[row] = origin + mean;
         float q = 0.f;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if ((u * L + l) * E < a.C) {
+            const bool in = (u * L + l) * E < a.C;
 #pragma unroll
-                for (int j = 0; j < E; ++j) {
-                    const float d = v[u][j] - mean;
-                    q += d * d;
-                }
+            for (int j = 0; j < E; ++j) {
+                v[u][j] -= mean;
+                if (in) q += v[u][j] * v[u][j];
             }
         }
         const float rstd = 1.0f / sqrtf(row_sum<L>(q, red, turn) * inv_c + a.eps);
-        if (l == 0 && a.mean) a.mean[row] = mean, a.rstd[row] = rstd;
+        if (l == 0 && a.mean) a.rstd[row] = rstd;
         T *y = (T *)a.y + row * (long long)a.C;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -100,7 +118,7 @@ __global__ __launch_bounds__(LN_THREADS) void ln_fwd_kernel(LnArgs a) {
             if (a.b) tok_load_param<T, E>(a.b, a.w32, c, b);
 #pragma unroll
             for (int j = 0; j < E; ++j) {
-                float o = (v[u][j] - mean) * rstd;
+                float o = v[u][j] * rstd;
                 if (a.w) o *= w[j];
                 if (a.b) o += b[j];
                 v[u][j] = o;
@@ -204,21 +222,22 @@ __global__ __launch_bounds__(LN_THREADS) void ln_fwd_long_kernel(LnArgs a) {
     const float inv_c = 1.0f / (float)a.C;
     for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T *x = (const T *)a.x + row * a.x_ld;
+        const float origin = ln_origin((float)x[0]);
         float s = 0.f, q = 0.f;
-        for (int c = threadIdx.x; c < a.C; c += LN_THREADS) s += (float)x[c];
+        for (int c = threadIdx.x; c < a.C; c += LN_THREADS) s += (float)x[c] - origin;
         const float mean = row_sum<LN_THREADS>(s, red, turn) * inv_c;
         for (int c = threadIdx.x; c < a.C; c += LN_THREADS) {
-            const float d = (float)x[c] - mean;
+            const float d = ((float)x[c] - origin) - mean;
             q += d * d;
         }
         const float rstd = 1.0f / sqrtf(row_sum<LN_THREADS>(q, red, turn) * inv_c + a.eps);
-        if (threadIdx.x == 0 && a.mean) a.mean[row] = mean, a.rstd[row] = rstd;
+        if (threadIdx.x == 0 && a.mean) a.mean[row] = origin + mean, a.rstd[row] = rstd;
         T *y = (T *)a.y + row * (long long)a.C;
         for (int c = threadIdx.x; c < a.C; c += LN_THREADS) {
             float w[1] = {1.f}, b[1] = {0.f};
             if (a.w) tok_load_param<T, 1>(a.w, a.w32, c, w);
             if (a.b) tok_load_param<T, 1>(a.b, a.w32, c, b);
-            y[c] = (T)(((float)x[c] - mean) * rstd * w[0] + b[0]);
+            y[c] = (T)((((float)x[c] - origin) - mean) * rstd * w[0] + b[0]);
         }
     }
 }

@@ -22,7 +22,7 @@ from . import token_ops as ops
 def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5) -> Tensor:
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension of ``x``.  ``weight`` and ``bias``, ``[C]``,
     are of x's type or float32 (both of one type), and so are their gradients.  A row of one channel or of equal channels
-    gives ``bias``."""
+    gives ``bias`` (for ``eps`` > 0)."""
     return (ops._binding or ops.binding()).layer_norm(x, weight, bias, eps)
 
 

@@ -55,3 +55,43 @@ def test_one_weight_at_an_odd_address(rows, c, dtype):
             assert torch.equal(got, w), moved
         with torch.no_grad():
             assert torch.equal(tokens.gated_ffn(x, *args, activation="relu"), y), moved
+
+
+# ---- layer norm around a large value -----------------------------------------------------------------------------------
+NORM_WIDTHS = [1, 3, 8, 50, 77, 129, 500, 999, 1000, 2048, 5001, 8192, 9001, 20000]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("c", NORM_WIDTHS)
+@pytest.mark.parametrize("value", [1000.1, 12345.6, -0.3, 7.0, 1e-30, 3e29])
+def test_layer_norm_of_equal_channels_is_the_bias(value, c, dtype):
+    if value == 3e29 and dtype == torch.float16:
+        value = 65504.0
+    x = torch.full((5, c), value, dtype=dtype, device=DEV).requires_grad_()
+    w, b = rnd(c, seed=20, dtype=dtype).requires_grad_(), rnd(c, seed=21, dtype=dtype).requires_grad_()
+    y = tokens.layer_norm(x, w, b)
+    assert torch.equal(y, b.detach().expand(5, c))
+    assert (tokens.layer_norm(x.detach()) == 0).all()
+    (dw,) = torch.autograd.grad(y, w, rnd(5, c, seed=22, dtype=dtype))
+    assert (dw == 0).all()
+
+
+@pytest.mark.parametrize("c", [c for c in NORM_WIDTHS if c > 1])
+@pytest.mark.parametrize("shift,scale", [(1000.1, 0.01), (12345.6, 0.5), (-3e5, 2.0), (0.5, 1.0)])
+def test_layer_norm_far_from_zero_keeps_its_precision(shift, scale, c):
+    """The rounding errors of y are those of the channels' distances from the row's first one, whatever is common to them: a sum
+    of n terms over 64 lanes and more is fewer than n / 64 + 24 roundings deep."""
+    rows, u = 6, 2.0 ** -24
+    x = rnd(rows, c, seed=23, scale=scale, shift=shift)
+    x[3] = 0.0
+    x[3, c // 2] = shift                                        # one channel apart, and its mirror: the first one apart
+    x[4] = 0.0
+    x[4, 0] = shift
+    y = tokens.layer_norm(x)
+    d = x.double()
+    rstd = 1 / (d.var(1, unbiased=False, keepdim=True) + 1e-5).sqrt()
+    xh = (d - d.mean(1, keepdim=True)) * rstd
+    far = (d - d[:, :1]).abs().amax(1, keepdim=True)
+    tol = u * (c / 64 + 24) * (far * rstd + xh.abs()) * 1.5 + 5 * u * xh.abs()
+    bad = (y.double() - xh).abs() > tol
+    assert not bad.any(), ((y.double() - xh).abs() / tol).max()
