@@ -583,11 +583,18 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
     float bias[8], bias2[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        // columns past the hidden width (up to the padded row) have zero products and no bias: they store zeros
         bias[j] = (EPI == TOK_EPI_GLU || EPI == TOK_EPI_STORE) && job.bias && n + j < job.N ? (float)((const T *)job.bias)[n + j] : 0.f;
         bias2[j] = EPI == TOK_EPI_GLU && p.bias_up && n + j < job.N ? (float)((const T *)p.bias_up)[n + j] : 0.f;
     }
     const bool in_n = n < n_stored;
+    // Hidden channels behind the last one are stored as zeros, whatever an infinity in x or dy makes of their zero weights: they
+    // are part of the units that the next product reads.
+    const bool ragged = EPI == TOK_EPI_GLU || EPI == TOK_EPI_GLU_GRAD ? n + 8 > job.N : false;
+    auto clear_behind = [&](float (&v)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (n + j >= job.N) v[j] = 0.f;
+    };
     // rows [r of the turned fragments], all of this lane's columns
     auto finish = [&](auto kind, long long m_first) {
         constexpr int KIND = decltype(kind)::value;
@@ -615,6 +622,7 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
                     float dg[8], du[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) dg[j] = v[j] * kd[k].value(j), du[j] = v[j] * ka[k].value(j);
+                    if (ragged) clear_behind(dg), clear_behind(du);
                     if constexpr (COL_SUMS) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j) col_sum[j] += dg[j], col_sum[8 + j] += du[j];
@@ -654,11 +662,13 @@ __device__ __forceinline__ void tok_gemm_body(const TokGemmArgs &p) {
                         tok_act_grad<EXACT, KIND>(v[j] + bias[j], v[j], da);
                         h[j] = v[j] * up, w[j] = up * da;
                     }
+                    if (ragged) clear_behind(v), clear_behind(w), clear_behind(h);
                     tok_keep8<T>(p.kept.a, p.kept.a_low, at, v);
                     tok_keep8<T>(p.kept.d, p.kept.d_low, at, w);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) h[j] = tok_act<EXACT, KIND>(v[j] + bias[j]) * (w[j] + bias2[j]);
+                    if (ragged) clear_behind(h);
                 }
                 tok_store8<T>((T *)p.h + at, h);
             } else if constexpr (EPI == TOK_EPI_PART) {

@@ -117,7 +117,8 @@ __device__ __forceinline__ void tok_narrow_body(const TokNarrowArgs &p) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) y[c][e] = 0.f;
 
-    auto chunk_product = [&](unsigned base) {
+    // `left`: hidden channels from the chunk's first one on
+    auto chunk_product = [&](unsigned base, int left) {
         tok_static_for<SUBS>([&](auto sub) {
             constexpr int SUB = decltype(sub)::value;
             tok_v4u fg[KS], fu[KS], fd[CB][2], bias[4];
@@ -164,6 +165,15 @@ __device__ __forceinline__ void tok_narrow_body(const TokNarrowArgs &p) {
             for (int e = 0; e < 16; ++e) h[e] = (T)(tok_act<false, KIND>(g[e]) * u[e]);
             tok_v4u fh[2];
             __builtin_memcpy(fh, h, 32);
+            // hidden channels behind the last one are zeros, whatever an infinity in x makes of their zero weights; element e is
+            // channel (e & 7) + 8 half + 16 (e >> 3) of the 32
+            if (left < (SUB + 1) * 32) {
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) {
+                    const int behind = SUB * 32 + (e & 7) + 8 * half + 16 * (e >> 3) - left;
+                    fh[e >> 3][(e & 7) >> 1] &= behind >= 0 ? 0u : behind == -1 ? 0x0000ffffu : 0xffffffffu;
+                }
+            }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
             for (int c = 0; c < CB; ++c) {
@@ -182,7 +192,7 @@ __device__ __forceinline__ void tok_narrow_body(const TokNarrowArgs &p) {
         asm volatile("" ::: "memory");
         if (c + 1 < chunks) copy(c + 1, (c + 1) & 1);
         const unsigned base = lds0 + (c & 1) * N::STAGE;
-        chunk_product(base);
+        chunk_product(base, p.F - c * HC);
     }
     __builtin_amdgcn_s_barrier();                            // the last chunk's copies have all landed (waited for above)
     asm volatile("" ::: "memory");

@@ -133,6 +133,8 @@ __device__ __forceinline__ void tok_rows_body(const TokRowsArgs &p) {
             else if (p.act == SR355_ACT_GELU) tok_act_grad<EXACT, SR355_ACT_GELU>(v[0], a, d);
             else if (p.act == SR355_ACT_RELU) tok_act_grad<EXACT, SR355_ACT_RELU>(v[0], a, d);
             else tok_act_grad<EXACT, SR355_ACT_SIGMOID>(v[0], a, d);
+            // (hidden channels behind the last one: zeros, whatever an infinity in x makes of their zero weights)
+            if (n >= p.N) a = d = v[Q - 1] = 0.f;
             const float h = a * v[Q - 1];
             const T high = (T)h;
             ((T *)p.out)[at] = high;

@@ -95,3 +95,33 @@ def test_layer_norm_far_from_zero_keeps_its_precision(shift, scale, c):
     tol = u * (c / 64 + 24) * (far * rstd + xh.abs()) * 1.5 + 5 * u * xh.abs()
     bad = (y.double() - xh).abs() > tol
     assert not bad.any(), ((y.double() - xh).abs() / tol).max()
+
+
+# ---- infinities ------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("c,f", [(24, 5), (24, 13), (8, 40), (100, 44), (24, 56), (264, 33)])
+@pytest.mark.parametrize("rows", [3, 70, 300, 16500])
+def test_an_infinity_beside_no_hidden_channels(rows, c, f, dtype):
+    """Hidden channels behind the last one, up to whole units and tiles, count for nothing: where the formula gives an infinity, it
+    is one.  All values are positive, so that the formula has no NaN."""
+    x = torch.ones(rows, c, dtype=dtype, device=DEV)
+    x[1, 2] = float("inf")
+    dy = torch.ones(rows, c, dtype=dtype, device=DEV)
+    ws = [torch.full(s, 0.125, dtype=dtype, device=DEV) for s in ((f, c), (f, c), (c, f))]
+    leaves = [v.detach().requires_grad_() for v in (x, *ws)]
+    y = tokens.gated_ffn(*leaves, activation="relu")
+    got = [y, *torch.autograd.grad(y, leaves, dy)]
+    with torch.no_grad():
+        got.append(tokens.gated_ffn(x, *ws, activation="relu"))
+    want = relu_block(x, dy, *ws)
+    u = torch.finfo(dtype).eps / 2
+    for k, (a, b) in enumerate(zip(got, (*want, want[0]))):
+        assert torch.equal(a.isinf(), b.to(dtype).isinf()) and not a.isnan().any(), k       # (fp16 ends at 65504)
+        ok = ~b.to(dtype).isinf()
+        assert ((a[ok].double() - b[ok]).abs() <= (3 * u + 2.0 ** -15) * b[ok]).all(), k
+    x[1, 2] = 1.0
+    dy[2, 1] = float("inf")
+    leaves = [v.detach().requires_grad_() for v in (x, *ws)]
+    got = torch.autograd.grad(tokens.gated_ffn(*leaves, activation="relu"), leaves, dy)
+    for k, (a, b) in enumerate(zip(got, relu_block(x, dy, *ws)[1:])):
+        assert torch.equal(a.isinf(), b.to(dtype).isinf()) and not a.isnan().any(), k
