@@ -159,10 +159,12 @@ __device__ __forceinline__ void tok_read(tok_v4u &f, tok_v2u &lo, tok_v2u &hi, u
 }
 
 // The activation and its derivative.  T = float goes through the exact functions, the 16-bit types through the hardware's
-// exp2 and reciprocal (errors of a few 2^-23, far below their own rounding) and, for the normal distribution's integral, the
-// polynomial of Abramowitz and Stegun 7.1.26: erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2) with t = 1 / (1 + p x), x >= 0, absolute
-// error at most 1.5e-7.  The library's erff takes some 45 instructions an element, which bounded the forward pass of
-// 262144 x 64 x 256 (130 us for the gate and up launch); this takes 15 and shares the exponential with the derivative.
+// exp2 and reciprocal (errors of a few 2^-23, far below their own rounding).  The normal distribution's integral is taken from
+// its small side, so that gelu keeps its relative precision where it is small: fp32 by erfc, the 16-bit types as density * t P(t)
+// with t = 1 / (1 + p |g|) and a polynomial of degree 6, a minimax fit that weighs the absolute error near zero and the relative one
+// behind (evaluated in fp32: 1.6e-7 and, down to g = -12.9, 8e-6; half a step of fp16 is 4.9e-4).  The library's erff takes some
+// 45 instructions an element, which bounded the forward pass of 262144 x 64 x 256 (130 us for the gate and up launch); this
+// takes 16 and shares the exponential with the derivative.
 template <bool EXACT>
 __device__ __forceinline__ float tok_sigmoid(float g) {
     if constexpr (EXACT) return 1.0f / (1.0f + expf(-g));
@@ -172,12 +174,13 @@ __device__ __forceinline__ float tok_sigmoid(float g) {
 template <bool EXACT>
 __device__ __forceinline__ void tok_normal(float g, float &cdf, float &density) {
     if constexpr (EXACT) {
-        cdf = 0.5f * (1.0f + erff(0.70710678118655f * g)), density = expf(-0.5f * g * g);
+        cdf = 0.5f * erfcf(-0.70710678118655f * g), density = expf(-0.5f * g * g);
     } else {
         density = __builtin_amdgcn_exp2f(-0.72134752044448f * g * g);
-        const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * 0.70710678118655f * fabsf(g));
-        const float poly = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-        const float tail = 0.5f * poly * density;
+        const float t = __builtin_amdgcn_rcpf(1.0f + 0.347788f * fabsf(g));
+        const float poly = 0.13893718f + t * (0.13539703f + t * (0.14573018f + t * (0.00086931005f + t * (0.22241315f +
+                           t * (-0.18805346f + t * 0.044706643f)))));
+        const float tail = t * poly * density;
         cdf = g < 0.f ? tail : 1.0f - tail;
     }
 }

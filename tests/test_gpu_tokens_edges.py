@@ -125,3 +125,31 @@ def test_an_infinity_beside_no_hidden_channels(rows, c, f, dtype):
     got = torch.autograd.grad(tokens.gated_ffn(*leaves, activation="relu"), leaves, dy)
     for k, (a, b) in enumerate(zip(got, relu_block(x, dy, *ws)[1:])):
         assert torch.equal(a.isinf(), b.to(dtype).isinf()) and not a.isnan().any(), k
+
+
+# ---- the activations far from zero ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [40, 300, 16500])
+def test_gelu_keeps_its_precision_where_it_is_small(rows, dtype):
+    """One channel and one hidden channel: y = gelu(x) * 4096 (fp16: 1024), its derivative beside it.  h is rounded to the type and taken over by
+    y, or y is rounded once; act' is kept with 16 bits; the normal integral itself is good to 2^-17 of its value."""
+    lo = -5.5 if dtype == torch.float16 else -12.0               # fp16: where 1024 gelu(x) is a normal number
+    x = torch.linspace(lo, 6.0, rows).to(dtype).to(DEV)[:, None].requires_grad_()
+    one = torch.ones(1, 1, dtype=dtype, device=DEV)
+    up = torch.full((1,), 4096.0 if dtype != torch.float16 else 1024.0, dtype=dtype, device=DEV)
+    d = x.detach().double()
+    cdf, density = 0.5 * torch.erfc(-d * 0.5 ** 0.5), torch.exp(-0.5 * d * d) / (2 * torch.pi) ** 0.5
+    want, slope = d * cdf * up.item(), (cdf + d * density) * up.item()
+    u = torch.finfo(dtype).eps / 2
+    # the exponent g^2 / 2 is rounded to fp32: relative to the result that is g^2 / 2 of its steps, twice
+    own = 2.0 ** -17 + 2.0 ** -23 * d * d
+    y = tokens.gated_ffn(x, one, torch.zeros_like(one), one, None, up, None, activation="gelu")
+    (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    with torch.no_grad():
+        alone = tokens.gated_ffn(x, one, torch.zeros_like(one), one, None, up, None, activation="gelu")
+    for got in (y, alone):
+        bad = (got.double() - want).abs() > (2 * u + own) * want.abs()
+        assert not bad.any(), (x[bad][0].item(), got[bad][0].item(), want[bad][0].item())
+    size = (cdf + (d * density).abs()) * up.item()
+    bad = (dx.double() - slope).abs() > 2 * u * slope.abs() + (own + (2.0 ** -15 if u > 2.0 ** -20 else 0.0)) * size
+    assert not bad.any(), (x[bad][0].item(), dx[bad][0].item(), slope[bad][0].item())
