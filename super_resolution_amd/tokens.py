@@ -11,9 +11,11 @@ be captured into a graph, and keep nothing between calls.  A training call that 
 autograd graph of the default stream still holds: PyTorch would add their gradients up there."""
 from __future__ import annotations
 
+import copy
 from typing import Optional
 
 import torch
+import torch.distributed as dist
 from torch import Tensor, nn
 
 from . import token_ops as ops
@@ -71,6 +73,10 @@ def blocked_from_rows(x: Tensor) -> Tensor:
     return x.reshape(N, H, W, units, 8).permute(0, 1, 3, 2, 4).contiguous()
 
 
+def _rank() -> int:
+    return dist.get_rank() if dist.is_available() and dist.is_initialized() else 0
+
+
 class FeedForwardBlock(nn.Module):
     """``x + dropout(gated_ffn(layer_norm(x)))`` on rows ``[..., channels]``: the channel-mixing half of a residual block.
 
@@ -78,7 +84,12 @@ class FeedForwardBlock(nn.Module):
     gradients come back as float32) and the normalisation's are used as they are.  In training mode with ``dropout > 0``
     every call takes the seed and step of ``rng_state`` (a buffer that checkpoints carry; ``seed()`` sets it) and advances
     the step, on the device, so that replays of a captured graph do too.  A forward pass that is run again for its gradients
-    (activation checkpointing) would take the next step and drop other elements: set ``rng_state`` back for it."""
+    (activation checkpointing) would take the next step and drop other elements: set ``rng_state`` back for it.
+
+    Every block starts with a seed of its own, drawn from PyTorch's default generator (``torch.manual_seed`` makes it
+    repeatable), and so does a ``deepcopy``, so stacked blocks drop different elements; blocks that are given one seed by
+    ``seed()`` or one ``state_dict`` drop the same.  The rank in ``torch.distributed``'s default group is dropout's ``site``:
+    replicas with equal seeds (DistributedDataParallel makes their buffers equal) drop different elements."""
 
     def __init__(self, channels: int, hidden: int, dropout: float = 0.0, activation: str = "silu", bias: bool = True,
                  eps: float = 1e-5):
@@ -91,6 +102,19 @@ class FeedForwardBlock(nn.Module):
         self.up = nn.Linear(channels, hidden, bias=bias)
         self.down = nn.Linear(hidden, channels, bias=bias)
         self.register_buffer("rng_state", torch.zeros(2, dtype=torch.int64))
+        self._draw_seed()
+
+    def _draw_seed(self) -> None:
+        with torch.no_grad():
+            self.rng_state[:1].random_(-(1 << 62), 1 << 62)
+            self.rng_state[1:].zero_()
+
+    def __deepcopy__(self, memo):
+        block = self.__class__.__new__(self.__class__)
+        memo[id(self)] = block
+        block.__dict__.update({k: copy.deepcopy(v, memo) for k, v in self.__dict__.items()})
+        block._draw_seed()
+        return block
 
     def seed(self, seed: int) -> None:
         """Start the dropout's generator at step 0 of ``seed``."""
@@ -114,4 +138,4 @@ class FeedForwardBlock(nn.Module):
             return x + h
         rng = self.rng_state.clone()          # what this call's backward pass reads, while the buffer moves on
         self.rng_state[1].add_(1)
-        return dropout(h, self.dropout, rng, residual=x)
+        return dropout(h, self.dropout, rng, _rank(), x)

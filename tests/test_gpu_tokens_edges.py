@@ -153,3 +153,16 @@ def test_gelu_keeps_its_precision_where_it_is_small(rows, dtype):
     size = (cdf + (d * density).abs()) * up.item()
     bad = (dx.double() - slope).abs() > 2 * u * slope.abs() + (own + (2.0 ** -15 if u > 2.0 ** -20 else 0.0)) * size
     assert not bad.any(), (x[bad][0].item(), dx[bad][0].item(), slope[bad][0].item())
+
+
+# ---- blocks ----------------------------------------------------------------------------------------------------------------
+def test_stacked_blocks_drop_different_elements():
+    """A dropped element is its skip.  Two masks of independent draws agree on 0.36 + 0.16 of n elements: five standard deviations."""
+    torch.manual_seed(31)
+    blocks = [tokens.FeedForwardBlock(64, 32, dropout=0.4).to(DEV) for _ in range(2)]
+    x, n = rnd(500, 64, seed=32), 500 * 64
+    drops = [b(x) == x for b in blocks] + [blocks[0](x) == x]
+    for k, a in enumerate(drops):
+        assert abs(int(a.sum()) - 0.4 * n) < 5 * (n * 0.24) ** 0.5
+        for b in drops[:k]:
+            assert abs(int((a == b).sum()) - 0.52 * n) < 5 * (n * 0.52 * 0.48) ** 0.5
