@@ -61,13 +61,20 @@ int code_of(at::ScalarType t) {
     return t == at::kBFloat16 ? SR355_DTYPE_BF16 : t == at::kHalf ? SR355_DTYPE_F16 : t == at::kFloat ? SR355_DTYPE_F32 : -1;
 }
 
+// (the kernels compute no tangents, so a dual tensor's derivative would be lost without a word)
+void check_dual(const char *who, const Tensor &t) {
+    TORCH_CHECK(!t._fw_grad(0).defined(), who, ": forward-mode derivatives are not supported (an input of shape ", t.sizes(), " carries a tangent)");
+}
+
 // x is a tensor of rows in one of the types
 void check_rows(const char *who, const Tensor &x) {
+    check_dual(who, x);
     TORCH_CHECK(x.is_cuda(), who, ": runs on ROCm devices only (got a tensor on ", x.device(), "); there is no CPU fallback");
     TORCH_CHECK(code_of(x.scalar_type()) >= 0, who, ": expected bfloat16, float16 or float32, got ", x.scalar_type());
     TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, who, ": expected rows of at least one channel, got shape ", x.sizes());
 }
 void check_device(const char *who, const Tensor &x, const Tensor &t) {
+    check_dual(who, t);
     TORCH_CHECK(t.device() == x.device(), who, ": tensors on ", x.device(), " and ", t.device());
 }
 

@@ -3,8 +3,10 @@ here."""
 import ctypes as C
 
 import pytest
+import torch
+import torch.autograd.forward_ad as fwd
 
-from super_resolution_amd import _lib
+from super_resolution_amd import _lib, tokens
 from super_resolution_amd._lib import FfnArgs
 
 
@@ -40,3 +42,13 @@ def test_gate_and_up_weights_are_padded_together(L, dtype, channels, rows, backw
     both = size(w_gate_dev=odd, w_up_dev=odd)
     assert both > size()
     assert size(w_gate_dev=odd) == both and size(w_up_dev=odd) == both
+
+
+def test_forward_mode_derivatives_are_refused():
+    """(They would be zero: the kernels compute no tangent.)"""
+    x, w, wd = torch.ones(4, 8), torch.ones(16, 8), torch.ones(8, 16)
+    rng = torch.zeros(2, dtype=torch.int64)
+    for call in (tokens.layer_norm, lambda t: tokens.gated_ffn(t, w, w, wd), lambda t: tokens.dropout(t, 0.5, rng),
+                 lambda t: torch.ops.sr355.layer_norm_fwd(t, None, None, 1e-5, False)):
+        with fwd.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            call(fwd.make_dual(x, torch.ones_like(x)))
