@@ -8,6 +8,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import subprocess
+import sys
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # SR355_LIB names another build of the same ABI (A/B measurements of kernel changes)
@@ -161,9 +162,9 @@ class Sr355Error(RuntimeError):
 
 
 def build(verbose: bool = False, again: bool = False) -> str:
-    """Compile libsr355.so for gfx950 with hipcc, and the binding beside it (works without a GPU); ``again``: also what is up
-    to date."""
-    cmd = ["make", "-C", CSRC_DIR, "-j8", *(["-B"] if again else [])]
+    """Compile libsr355.so for gfx950 with hipcc, and the binding beside it for the interpreter that runs this (works without a
+    GPU); ``again``: also what is up to date."""
+    cmd = ["make", "-C", CSRC_DIR, "-j8", f"PYTHON={sys.executable or 'python3'}", *(["-B"] if again else [])]
     res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if verbose or res.returncode:
         print(res.stdout)

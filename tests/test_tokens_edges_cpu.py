@@ -1,6 +1,8 @@
 """CPU: the operators on rows of channels where a call's arguments, not its numbers, decide what happens.  No kernel runs
 here."""
 import ctypes as C
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -52,3 +54,12 @@ def test_forward_mode_derivatives_are_refused():
                  lambda t: torch.ops.sr355.layer_norm_fwd(t, None, None, 1e-5, False)):
         with fwd.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
             call(fwd.make_dual(x, torch.ones_like(x)))
+
+
+def test_the_binding_is_built_for_the_running_interpreter(monkeypatch):
+    """Its headers, its libraries and its C++ ABI are those of the PyTorch that will load it, whatever python3 is on PATH."""
+    asked = []
+    monkeypatch.setattr(_lib.subprocess, "run", lambda cmd, **kw: asked.append(cmd) or subprocess.CompletedProcess(cmd, 0, ""))
+    _lib.build()
+    _lib.build(again=True)
+    assert len(asked) == 2 and all(f"PYTHON={sys.executable}" in cmd for cmd in asked)
