@@ -352,7 +352,7 @@ int sr355_loss_fwd(const float *a_dev, const float *b_dev, float b_const, size_t
  * and of a fixed order.  Any sizes, strides and alignment are taken; widths, strides and pointers that are multiples of 16
  * bytes run on 16-byte accesses. */
 
-/* y = (x - mean) / sqrt(var + eps) * w + b over the C channels of each row.  w and b may be null; they are of the
+/* y = (x - mean) / sqrt(var + eps) * w + b over the C channels (at most 2^31 - 256) of each row.  w and b may be null; they are of the
  * activations' type or fp32 (w_dtype).  mean / rstd [rows] fp32 for the backward pass (both null: not written). */
 int sr355_layer_norm_fwd(const void *x_dev, long long rows, int C, long long x_ld, int dtype, const void *w_dev,
                          const void *b_dev, int w_dtype, float eps, void *y_dev, float *mean_dev, float *rstd_dev,

@@ -9,6 +9,8 @@
 // of 32768 x 1024 bf16's 26).  The backward pass takes the mean as it is stored, rounded to fp32.  Statistics, sums and the two
 // row means are fp32.  The backward pass keeps dw / db of the lane's columns in registers over all rows of the workgroup and
 // writes one partial row per workgroup; a second launch adds the partials in order.  No atomics.
+#include <climits>
+
 #include "token_common.h"
 
 namespace sr355 {
@@ -16,6 +18,7 @@ namespace sr355 {
 namespace {
 constexpr int LN_THREADS = 256;
 constexpr int LN_MAX_PARTS = 512;      // two workgroups per CU
+constexpr int LN_MOST = INT_MAX - 255; // channels: a thread's index steps by 256 behind the last one
 constexpr int LN_LONG = 8192;          // channels from which on no type's row fits a workgroup's registers
 
 // Partial rows of dw and db, at most: rows beyond the registers have columns enough to fill the chip with fewer.
@@ -295,26 +298,30 @@ struct SumArgs {
     int n_parts, out_dtype;
 };
 constexpr int SUM_WAVES = 16;
+constexpr int SUM_WGS = 1 << 21;       // a grid axis holds fewer than 2^32 threads (more are dropped without an error)
 __global__ __launch_bounds__(64 * SUM_WAVES) void tok_sum_parts_kernel(SumArgs a) {
     __shared__ float red[SUM_WAVES][64];
     const int k = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int j = blockIdx.x * 64 + lane;
-    float s = 0.f;
-    if (j < a.count[k]) {
-        const float *p = a.parts + a.first[k] + j;
-        const int lo = (int)((long long)a.n_parts * wave / SUM_WAVES), hi = (int)((long long)a.n_parts * (wave + 1) / SUM_WAVES);
+    for (long long first = blockIdx.x * 64LL; first < a.count[k]; first += gridDim.x * 64LL) {
+        const long long j = first + lane;
+        float s = 0.f;
+        if (j < a.count[k]) {
+            const float *p = a.parts + a.first[k] + j;
+            const int lo = (int)((long long)a.n_parts * wave / SUM_WAVES), hi = (int)((long long)a.n_parts * (wave + 1) / SUM_WAVES);
 #pragma unroll 8
-        for (int i = lo; i < hi; ++i) s += p[(size_t)i * a.stride];
-    }
-    red[wave][lane] = s;
-    __syncthreads();
-    if (wave || j >= a.count[k]) return;
-    s = 0.f;
+            for (int i = lo; i < hi; ++i) s += p[(size_t)i * a.stride];
+        }
+        __syncthreads();                                    // (the columns before these have been added)
+        red[wave][lane] = s;
+        __syncthreads();
+        if (wave || j >= a.count[k]) continue;
+        s = 0.f;
 #pragma unroll
-    for (int w = 0; w < SUM_WAVES; ++w) s += red[w][lane];
-    if (a.out_dtype == SR355_DTYPE_F32) ((float *)a.out[k])[j] = s;
-    else if (a.out_dtype == SR355_DTYPE_BF16) ((bf16_t *)a.out[k])[j] = (bf16_t)s;
-    else ((f16_t *)a.out[k])[j] = (f16_t)s;
+        for (int w = 0; w < SUM_WAVES; ++w) s += red[w][lane];
+        if (a.out_dtype == SR355_DTYPE_F32) ((float *)a.out[k])[j] = s;
+        else if (a.out_dtype == SR355_DTYPE_BF16) ((bf16_t *)a.out[k])[j] = (bf16_t)s;
+        else ((f16_t *)a.out[k])[j] = (f16_t)s;
+    }
 }
 
 int ln_grid(long long rows, int rows_per_wg, int most) {
@@ -396,9 +403,9 @@ bool ln_vec(int dtype, int C, long long ld0, long long ld1, const void *p0, cons
 }
 
 bool ln_args_ok(const char *who, long long rows, int C, int dtype, long long ld0, long long ld1, const void *w, int w_dtype) {
-    if (rows < 0 || C < 1 || !tok_dtype_ok(dtype) || ld0 < C || ld1 < C ||
+    if (rows < 0 || C < 1 || C > LN_MOST || !tok_dtype_ok(dtype) || ld0 < C || ld1 < C ||
         (w && w_dtype != dtype && w_dtype != SR355_DTYPE_F32)) {
-        set_error("%s: bad arguments (rows=%lld C=%d dtype=%d, row strides %lld and %lld elements, parameters of type %d: the "
+        set_error("%s: bad arguments (rows=%lld, C=%d channels of at most 2^31 - 256, dtype=%d, row strides %lld and %lld elements, parameters of type %d: the "
                   "activations' type or fp32)", who, rows, C, dtype, ld0, ld1, w_dtype);
         return false;
     }
@@ -418,7 +425,8 @@ int launch_tok_sum_parts(const float *parts, int n_parts, long long stride, cons
         ++n;
     }
     if (n == 0 || most == 0) return SR355_OK;
-    hipLaunchKernelGGL(tok_sum_parts_kernel, dim3((unsigned)tok_cdiv(most, 64), n), dim3(64 * SUM_WAVES), 0, stream, s);
+    const long long wgs = tok_cdiv(most, 64);
+    hipLaunchKernelGGL(tok_sum_parts_kernel, dim3((unsigned)(wgs < SUM_WGS ? wgs : SUM_WGS), n), dim3(64 * SUM_WAVES), 0, stream, s);
     return check_hip(hipGetLastError(), "column sum launch");
 }
 
@@ -444,8 +452,8 @@ int sr355_layer_norm_fwd(const void *x, long long rows, int C, long long x_ld, i
 }
 
 size_t sr355_layer_norm_bwd_workspace_bytes(int C) {
-    if (C < 1) {
-        set_error("layer_norm_bwd_workspace_bytes: C=%d", C);
+    if (C < 1 || C > LN_MOST) {
+        set_error("layer_norm_bwd_workspace_bytes: C=%d channels", C);
         return 0;
     }
     return (size_t)ln_max_parts(C) * 2 * C * sizeof(float);

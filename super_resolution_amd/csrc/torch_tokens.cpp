@@ -14,6 +14,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <array>
+#include <climits>
 #include <map>
 #include <optional>
 #include <string>
@@ -157,6 +158,9 @@ variable_list once(variable_list grads, const char *who) {
 }
 
 // ---- layer norm ----------------------------------------------------------------------------------------------------
+void check_channels(const char *who, const Tensor &x) {
+    TORCH_CHECK(x.size(-1) <= INT_MAX - 255, who, ": ", x.size(-1), " channels; up to 2^31 - 256 are supported");
+}
 struct NormParams {
     Tensor w, b;
     at::ScalarType type;
@@ -171,6 +175,7 @@ struct NormParams {
 
 std::tuple<Tensor, Tensor> layer_norm_fwd(const Tensor &x, const OptTensor &weight, const OptTensor &bias, double eps, bool want_stats) {
     check_rows("layer_norm", x);
+    check_channels("layer_norm", x);
     const NormParams p("layer_norm", x, weight, bias);
     TORCH_CHECK(eps >= 0.0, "layer_norm: eps must not be negative, got ", eps);
     const Rows r(x);
@@ -179,7 +184,6 @@ std::tuple<Tensor, Tensor> layer_norm_fwd(const Tensor &x, const OptTensor &weig
     Tensor y = at::empty(x.sizes(), x.options());
     Tensor stats = at::empty(want_stats ? std::vector<int64_t>{2, rows} : std::vector<int64_t>{0}, x.options().dtype(at::kFloat));
     float *s = want_stats && rows ? stats.mutable_data_ptr<float>() : nullptr;
-    TORCH_CHECK(c <= INT_MAX, "layer_norm: too many channels");
     ok(api.layer_norm_fwd(r.data(), rows, static_cast<int>(c), r.ld, code_of(x.scalar_type()), ptr(p.w), ptr(p.b), code_of(p.type),
                           static_cast<float>(eps), y.mutable_data_ptr(), s, s ? s + rows : nullptr, launch.stream),
        "sr355_layer_norm_fwd");
@@ -190,6 +194,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor &dy, const Tensor
                                                   at::ScalarType param_type, const std::vector<bool> &need) {
     const char *who = "layer_norm backward";
     check_rows(who, x);
+    check_channels(who, x);
     check_device(who, x, dy);
     check_device(who, x, stats);
     const int64_t c = x.size(-1), rows = x.numel() / c;

@@ -182,3 +182,37 @@ def test_forward_mode_derivatives_are_refused():
         with fwd.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
             call()
             pytest.fail(f"call {k} was not refused")
+
+
+# ---- layer norm of very long rows ------------------------------------------------------------------------------------------
+def test_layer_norm_of_a_row_of_more_than_2_28_channels():
+    """One row, so that db is dy and dw one product; the two row means are sums of 2^20 terms a lane."""
+    c, u, step = (1 << 28) + 70, 2.0 ** -8, 2.0 ** -24
+    g = torch.Generator(DEV).manual_seed(40)
+    x, dy, w = (torch.randn(c, device=DEV, generator=g).to(torch.bfloat16) for _ in range(3))
+    leaves = [x[None].requires_grad_(), w.requires_grad_(), torch.zeros(c, dtype=torch.bfloat16, device=DEV, requires_grad=True)]
+    y = tokens.layer_norm(*leaves)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy[None])
+    assert torch.equal(db, dy)
+    deep = step * (c / 256 + 24)
+    with torch.no_grad():
+        d = x.double()
+        d -= d.mean()
+        rstd = (d.square().mean() + 1e-5).rsqrt()
+        d *= rstd                                                  # xh: of size one, its mean and scale off by `deep` at most
+        want = d * w.double()
+        assert ((y[0].double() - want).abs() <= (u + 4 * deep) * want.abs() + 4 * deep * w.double().abs()).all()
+        want = d * dy.double()
+        assert ((dw.double() - want).abs() <= (u + 4 * deep) * want.abs() + 4 * deep * dy.double().abs()).all()
+        t = dy.double() * w.double()
+        s, q, size = t.mean(), (t * d).mean(), t.abs().mean()
+        want = rstd * (t - s - d * q)
+        assert ((dx[0].double() - want).abs() <= (u + 4 * deep) * want.abs() + 8 * deep * size * (1 + d.abs())).all()
+
+
+def test_layer_norm_refuses_more_channels_than_an_int_counts():
+    x, stats = torch.zeros(1, 1, device=DEV).expand(1, (1 << 32) + 8), torch.zeros(2, 1, device=DEV)
+    with pytest.raises(RuntimeError, match="channels"):
+        tokens.layer_norm(x)
+    with pytest.raises(RuntimeError, match="channels"):
+        torch.ops.sr355.layer_norm_bwd(x, x, None, stats, torch.float32, [True, False, False])

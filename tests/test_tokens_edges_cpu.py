@@ -63,3 +63,14 @@ def test_the_binding_is_built_for_the_running_interpreter(monkeypatch):
     _lib.build()
     _lib.build(again=True)
     assert len(asked) == 2 and all(f"PYTHON={sys.executable}" in cmd for cmd in asked)
+
+
+def test_layer_norm_counts_channels_without_overflow(L):
+    """A thread steps 256 channels at a time behind the last one, in an int."""
+    last = 2 ** 31 - 1
+    for c in (last, last - 254):
+        assert L.sr355_layer_norm_fwd(P, 1, c, c, 0, None, None, 0, 1e-5, P, None, None, None) == -1
+        assert L.sr355_layer_norm_bwd(P, c, P, c, 1, c, 0, None, 0, P, P, P, None, None, None, 0, None) == -1
+        assert b"channels" in L.sr355_last_error()
+        assert L.sr355_layer_norm_bwd_workspace_bytes(c) == 0
+    assert L.sr355_layer_norm_bwd_workspace_bytes(last - 255) > 0
