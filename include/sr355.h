@@ -370,7 +370,8 @@ int sr355_layer_norm_bwd(const void *dy_dev, long long dy_ld, const void *x_dev,
 int sr355_dropout(const void *x_dev, const void *skip_dev, long long n, int dtype, double p, const long long *rng_dev,
                   unsigned site, void *y_dev, void *stream);
 
-/* Gated feed-forward block: y = (act(x Wg' + bg) * (x Wu' + bu)) Wd' + bd. */
+/* Gated feed-forward block: y = (act(x Wg' + bg) * (x Wu' + bu)) Wd' + bd.  Widths up to 2^20, fewer than 2^31 rows, and fewer
+ * tiles of rows and hidden channels than one launch has (2^24 of at least 128 x 32). */
 #define SR355_ACT_SILU 0
 #define SR355_ACT_GELU 1    /* g * Phi(g), by erf */
 #define SR355_ACT_RELU 2

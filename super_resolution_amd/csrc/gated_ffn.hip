@@ -12,6 +12,8 @@
 //
 // Operands are read 16 bytes at a time.  What does not allow that (a width, stride or pointer that is no multiple of 16
 // bytes) is first copied into padded rows of the workspace, one launch for all of them.
+#include <climits>
+
 #include "token_narrow.h"
 #include "token_rows.h"
 
@@ -128,6 +130,11 @@ __global__ __launch_bounds__(256) void reduce_splits_kernel(ReduceArgs a) {
 
 template <typename T, typename G, bool A_RC, bool B_RC, int EPI, bool SUMS = false>
 int gemm_launch(const TokGemmArgs &g, const char *what, hipStream_t stream) {
+    // (a grid axis holds fewer than 2^32 threads; the runtime drops more without an error)
+    if ((long long)g.n_tiles * g.splits * G::THREADS > 0xffffffffLL) {
+        set_error("%s: too many tiles for one launch", what);
+        return SR355_ERR_INVALID;
+    }
     void (*const kernel)(TokGemmArgs) = tok_gemm_kernel<T, G, A_RC, B_RC, EPI, SUMS>;
     if (G::LDS_BYTES > 64 * 1024) {
         // (per device, and cheap: not remembered)
@@ -147,7 +154,7 @@ long long set_tiles(TokGemmArgs &g, bool glu) {
         g.job[j].tiles_n = (int)tok_cdiv(g.job[j].N, glu ? G::BN / 2 : G::BN);
         n += (long long)g.job[j].tiles_m * g.job[j].tiles_n;
     }
-    g.n_tiles = (int)n;
+    g.n_tiles = (int)(n < INT_MAX ? n : INT_MAX);
     return n;
 }
 
@@ -166,10 +173,7 @@ int gemm_pick(TokGemmArgs &g, const char *what, hipStream_t stream) {
         if (small <= N_CU) return gemm_launch<T, TileFew, A_RC, B_RC, EPI, SUMS>(g, what, stream);
         if (tiles_are_big(set_tiles<Tile256>(g, glu), small)) return gemm_launch<T, Tile256, A_RC, B_RC, EPI, SUMS>(g, what, stream);
     }
-    if (set_tiles<TileSmall<T>>(g, glu) > 0x3fffffffLL) {
-        set_error("%s: too many tiles", what);
-        return SR355_ERR_INVALID;
-    }
+    set_tiles<TileSmall<T>>(g, glu);
     return gemm_launch<T, TileSmall<T>, A_RC, B_RC, EPI, SUMS>(g, what, stream);
 }
 

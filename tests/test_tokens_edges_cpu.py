@@ -74,3 +74,12 @@ def test_layer_norm_counts_channels_without_overflow(L):
         assert b"channels" in L.sr355_last_error()
         assert L.sr355_layer_norm_bwd_workspace_bytes(c) == 0
     assert L.sr355_layer_norm_bwd_workspace_bytes(last - 255) > 0
+
+
+@pytest.mark.parametrize("dtype,rows,hidden", [(_lib.DTYPE_F32, 1 << 30, 72), (_lib.DTYPE_BF16, 0x7fffff00, 264), (_lib.DTYPE_F16, 1 << 30, 1 << 20)])
+def test_gated_ffn_refuses_more_tiles_than_a_grid_has(L, dtype, rows, hidden):
+    """A launch of 2^32 threads or more would leave out what is beyond."""
+    call = lambda: ffn(dtype=dtype, rows=rows, channels=8, hidden=hidden, workspace_bytes=1 << 62, saved_bytes=1 << 62, dw_up_dev=P)
+    for entry in (L.sr355_gated_ffn_fwd, L.sr355_gated_ffn_bwd):
+        assert entry(call(), None) == -1
+        assert b"too many tiles" in L.sr355_last_error()
