@@ -9,6 +9,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
@@ -18,6 +19,7 @@
 #include <map>
 #include <optional>
 #include <string>
+#include <unordered_set>
 #include <vector>
 
 #include "../../include/sr355.h"
@@ -119,16 +121,30 @@ struct Launch {                       // the tensors' device is current and its 
 Tensor scratch(const Tensor &x, size_t bytes) { return at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte)); }
 
 // A leaf's gradients are added up on the stream that was current when the oldest live graph of the leaf was recorded.  In a
-// capture that must not be the default stream: the engine would make it wait for the captured one, which ends the process.
+// capture that must not be the default stream: the engine would make it wait for the captured one, which ends the process.  The
+// leaves of a call are those among its inputs and those that the others were made from.
 void check_capture(const std::vector<Tensor> &inputs) {
+    std::vector<torch::autograd::Node *> ahead;
+    std::vector<std::shared_ptr<torch::autograd::Node>> held;
     for (const Tensor &t : inputs) {
-        if (!t.defined() || !t.is_cuda() || !t.requires_grad() || !t.is_leaf()) continue;
+        if (!t.defined() || !t.is_cuda() || !t.requires_grad()) continue;
         const c10::OptionalDeviceGuard guard(t.device());
         if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
-        const auto stream = node ? node->stream() : std::nullopt;
-        TORCH_CHECK(!stream || stream->id() != 0, "a graph is being captured, and a leaf of shape ", t.sizes(),
-                    " still belongs to one that was recorded on the default stream: drop that graph's outputs first");
+        held.push_back(t.is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(t) : t.grad_fn());
+        if (held.back()) ahead.push_back(held.back().get());
+    }
+    std::unordered_set<const torch::autograd::Node *> seen;
+    while (!ahead.empty()) {
+        const auto *node = ahead.back();
+        ahead.pop_back();
+        if (!seen.insert(node).second) continue;
+        if (const auto *leaf = dynamic_cast<const torch::autograd::AccumulateGrad *>(node)) {
+            const auto stream = const_cast<torch::autograd::AccumulateGrad *>(leaf)->stream();
+            TORCH_CHECK(!stream || stream->id() != 0, "a graph is being captured, and a leaf of shape ", leaf->variable.sizes(),
+                        " still belongs to one that was recorded on the default stream: drop that graph's outputs first");
+        }
+        for (const auto &edge : node->next_edges())
+            if (edge.is_valid()) ahead.push_back(edge.function.get());
     }
 }
 // whether autograd records a call with these inputs
@@ -419,7 +435,6 @@ PYBIND11_MODULE(_torch_tokens, m) {
     namespace py = pybind11;
     typedef py::call_guard<py::gil_scoped_release> free;
     m.def("connect", &connect);
-    m.def("check_capture", &check_capture);
     m.def("layer_norm", &layer_norm, free());
     m.def("dropout", &dropout, free());
     m.def("gated_ffn", &gated_ffn, free());

@@ -7,8 +7,9 @@ fp32 sums of a fixed order; ``FeedForwardBlock`` composes them into the channel-
 
 Any sizes, leading dimensions and strides are taken; what is not laid out as rows of contiguous channels is copied first.
 Widths that are multiples of 16 bytes are the fast ones.  All calls run on the current stream of their tensors' device, can
-be captured into a graph, and keep nothing between calls.  A training call that is captured refuses leaves that a live
-autograd graph of the default stream still holds: PyTorch would add their gradients up there."""
+be captured into a graph, and keep nothing between calls.  A training call that is captured refuses leaves, its own and those
+that its inputs were made from, that a live autograd graph of the default stream still holds: PyTorch would add their gradients
+up there."""
 from __future__ import annotations
 
 import copy
@@ -124,9 +125,6 @@ class FeedForwardBlock(nn.Module):
     def forward(self, x: Tensor) -> Tensor:
         if x.dim() < 1 or x.shape[-1] != self.channels:
             raise RuntimeError(f"FeedForwardBlock: expected rows of {self.channels} channels, got {tuple(x.shape)}")
-
-        if torch.is_grad_enabled() and x.is_cuda and torch.cuda.is_current_stream_capturing():
-            ops.binding().check_capture([x, *self.parameters()])     # (the calls see the parameters' copies in x's type)
 
         def typed(t: Optional[Tensor]) -> Optional[Tensor]:
             return None if t is None else t.to(x.dtype)

@@ -216,3 +216,36 @@ def test_layer_norm_refuses_more_channels_than_an_int_counts():
         tokens.layer_norm(x)
     with pytest.raises(RuntimeError, match="channels"):
         torch.ops.sr355.layer_norm_bwd(x, x, None, stats, torch.float32, [True, False, False])
+
+
+# ---- captures ----------------------------------------------------------------------------------------------------------------
+def test_a_capture_sees_leaves_behind_other_operations():
+    """Parameters that are cast for the call, or an input that other layers made: their leaves' gradients are added up by PyTorch,
+    too, on the stream of the graph that lives."""
+    x, w = rnd(20, 16, seed=50, dtype=torch.bfloat16), rnd(16, seed=51, shift=1.0).requires_grad_()
+    ws = [rnd(*s, seed=52 + k, scale=0.2).requires_grad_() for k, s in enumerate(((40, 16), (40, 16), (16, 40)))]
+    rng = torch.zeros(2, dtype=torch.int64, device=DEV)
+    half = lambda t: t.to(torch.bfloat16)
+    calls = (lambda: tokens.layer_norm(x, half(w)), lambda: tokens.gated_ffn(x, *map(half, ws)),
+             lambda: tokens.layer_norm(x * half(w) + 1.0), lambda: tokens.dropout(x * half(w), 0.5, rng))
+    leaves = ([w], ws, [w], [w])
+    want = [torch.autograd.grad(c().float().sum(), v) for c, v in zip(calls, leaves)]
+    live = [c() for c in calls]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in calls:
+            with pytest.raises(RuntimeError, match="recorded on the default stream"):
+                call()
+        out = x * 2
+    graph.replay()
+    assert torch.equal(out, x * 2)
+    live.clear()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [torch.autograd.grad(c().float().sum(), v) for c, v in zip(calls, leaves)]
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
+        torch.cuda.synchronize()
