@@ -2,7 +2,8 @@
 and dropout onto a skip (csrc/layer_norm.hip, gated_ffn.hip, dropout.hip behind the C ABI of libsr355.so).
 
 Argument checks, memory, streams and autograd are in ``_torch_tokens.so`` (csrc/torch_tokens.cpp), built beside the library;
-the functions that a program calls are in ``tokens``."""
+the functions that a program calls are in ``tokens``.  They go to the binding's own autograd nodes, and to these ops where
+PyTorch has to see an operator: in ``torch.compile`` and ``torch.export``, with fake tensors and under dispatch modes."""
 from __future__ import annotations
 
 import ctypes as C
@@ -14,9 +15,8 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import DTYPE_BF16, DTYPE_F16, DTYPE_F32, FfnArgs, Sr355Error
+from ._lib import Sr355Error
 
-CODES = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16, torch.float32: DTYPE_F32}
 ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}     # SR355_ACT_* of include/sr355.h
 BINDING_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_torch_tokens.so")
 
@@ -59,6 +59,25 @@ def _(x, weight, bias, eps, want_stats):
     return (x.new_empty(x.shape), x.new_empty((2, rows) if want_stats else (0,), dtype=torch.float32))
 
 
+def _norm_context(ctx, inputs, output):
+    x, weight, bias, eps, want_stats = inputs
+    ctx.save_for_backward(x, weight, output[1] if want_stats else None)
+    ctx.eps = eps
+    ctx.param_dtype = next((t.dtype for t in (weight, bias) if t is not None), torch.float32)
+
+
+def _norm_backward(ctx, dy, _):
+    x, weight, stats = ctx.saved_tensors
+    if stats is None:                     # (a caller of the op who did not ask for them)
+        stats = torch.ops.sr355.layer_norm_fwd(x, weight, None, ctx.eps, True)[1]
+    need = list(ctx.needs_input_grad[:3])
+    grads = torch.ops.sr355.layer_norm_bwd(dy, x, weight, stats, ctx.param_dtype, need)
+    return (*(g if n else None for g, n in zip(grads, need)), None, None)
+
+
+layer_norm_fwd.register_autograd(_norm_backward, setup_context=_norm_context)
+
+
 @torch.library.custom_op("sr355::layer_norm_bwd", mutates_args=())
 def layer_norm_bwd(dy: Tensor, x: Tensor, weight: Optional[Tensor], stats: Tensor, param_dtype: torch.dtype,
                    need: List[bool]) -> Tuple[Tensor, Tensor, Tensor]:
@@ -85,6 +104,19 @@ def _(x, skip, p, rng, site):
     return x.new_empty(x.shape)
 
 
+def _dropout_context(ctx, inputs, output):
+    _, _, ctx.p, rng, ctx.site = inputs
+    ctx.save_for_backward(rng)
+
+
+def _dropout_backward(ctx, dy):
+    dx = torch.ops.sr355.dropout(dy, None, ctx.p, ctx.saved_tensors[0], ctx.site) if ctx.needs_input_grad[0] else None
+    return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
+
+
+dropout.register_autograd(_dropout_backward, setup_context=_dropout_context)
+
+
 @torch.library.custom_op("sr355::gated_ffn_fwd", mutates_args=())
 def gated_ffn_fwd(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, b_gate: Optional[Tensor],
                   b_up: Optional[Tensor], b_down: Optional[Tensor], activation: int,
@@ -96,11 +128,35 @@ def gated_ffn_fwd(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, b_gat
 
 @gated_ffn_fwd.register_fake
 def _(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation, want_saved):
-    a = FfnArgs()
-    a.dtype, a.activation, a.channels, a.hidden = CODES[x.dtype], activation, x.shape[-1], w_gate.shape[0]
-    a.rows, a.x_ld = x.numel() // x.shape[-1], x.shape[-1]
-    size = _lib.lib().sr355_gated_ffn_saved_bytes(C.byref(a)) if want_saved else 0
+    size = saved_bytes(x.numel() // x.shape[-1], w_gate.shape[0], x.dtype) if want_saved else 0
     return x.new_empty(x.shape), x.new_empty((size,), dtype=torch.uint8)
+
+
+def saved_bytes(rows, hidden: int, dtype: torch.dtype):
+    """``sr355_gated_ffn_saved_bytes``, for a number of rows that may be symbolic."""
+    e = dtype.itemsize
+    line = 128 // e
+    step = line if hidden >= 4 * line else 8
+    n = rows * ((hidden + step - 1) // step * step)
+    whole = lambda b: (b + 255) // 256 * 256
+    return 3 * whole(n * e) + (2 * whole(n) if e == 2 else 0) + 256
+
+
+def _ffn_context(ctx, inputs, output):
+    x, w_gate, w_up, w_down, b_gate, b_up, b_down, ctx.activation, want_saved = inputs
+    ctx.save_for_backward(x, w_gate, w_up, w_down, b_gate, b_up, output[1] if want_saved else None)
+
+
+def _ffn_backward(ctx, dy, _):
+    x, w_gate, w_up, w_down, b_gate, b_up, saved = ctx.saved_tensors
+    if saved is None:                     # (a caller of the op who did not ask for it)
+        saved = torch.ops.sr355.gated_ffn_fwd(x, w_gate, w_up, w_down, b_gate, b_up, None, ctx.activation, True)[1]
+    need = list(ctx.needs_input_grad[:7])
+    grads = torch.ops.sr355.gated_ffn_bwd(dy, x, w_gate, w_up, w_down, saved, ctx.activation, need)
+    return (*(g if n else None for g, n in zip(grads, need)), None, None)
+
+
+gated_ffn_fwd.register_autograd(_ffn_backward, setup_context=_ffn_context)
 
 
 @torch.library.custom_op("sr355::gated_ffn_bwd", mutates_args=())

@@ -22,11 +22,22 @@ from torch import Tensor, nn
 from . import token_ops as ops
 
 
+def _recorded(*tensors: Optional[Tensor]) -> bool:
+    """Whether autograd records a call with these inputs."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# Each function asks the binding, which answers with nothing where PyTorch has to see an operator (a compiler that traces this code
+# is told apart here): then the registered op is called.
 def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5) -> Tensor:
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension of ``x``.  ``weight`` and ``bias``, ``[C]``,
     are of x's type or float32 (both of one type), and so are their gradients.  A row of one channel or of equal channels
     gives ``bias`` (for ``eps`` > 0)."""
-    return (ops._binding or ops.binding()).layer_norm(x, weight, bias, eps)
+    if not torch.compiler.is_dynamo_compiling():
+        y = (ops._binding or ops.binding()).layer_norm(x, weight, bias, eps)
+        if y is not None:
+            return y
+    return torch.ops.sr355.layer_norm_fwd(x, weight, bias, eps, _recorded(x, weight, bias))[0]
 
 
 def dropout(x: Tensor, p: float, rng: Tensor, site: int = 0, residual: Optional[Tensor] = None) -> Tensor:
@@ -39,7 +50,11 @@ def dropout(x: Tensor, p: float, rng: Tensor, site: int = 0, residual: Optional[
     it runs, so a captured graph's replays drop what the words say then; changing them in place between a call and its
     backward pass is an error that autograd reports.  ``p`` counts in steps of 2^-16 and the scale is that of the nearest
     step; a dropped infinity or NaN is dropped."""
-    return (ops._binding or ops.binding()).dropout(x, p, rng, site, residual)
+    if not torch.compiler.is_dynamo_compiling():
+        y = (ops._binding or ops.binding()).dropout(x, p, rng, site, residual)
+        if y is not None:
+            return y
+    return torch.ops.sr355.dropout(x, residual, p, rng, site)
 
 
 def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, b_gate: Optional[Tensor] = None,
@@ -51,7 +66,12 @@ def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, b_gate: O
     hidden channel of every row of x."""
     if activation not in ops.ACTIVATIONS:
         raise RuntimeError(f"gated_ffn: activation must be one of {', '.join(ops.ACTIVATIONS)}, got {activation!r}")
-    return (ops._binding or ops.binding()).gated_ffn(x, w_gate, w_up, w_down, b_gate, b_up, b_down, ops.ACTIVATIONS[activation])
+    if not torch.compiler.is_dynamo_compiling():
+        y = (ops._binding or ops.binding()).gated_ffn(x, w_gate, w_up, w_down, b_gate, b_up, b_down, ops.ACTIVATIONS[activation])
+        if y is not None:
+            return y
+    return torch.ops.sr355.gated_ffn_fwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, ops.ACTIVATIONS[activation],
+                                         _recorded(x, w_gate, w_up, w_down, b_gate, b_up, b_down))[0]
 
 
 def rows_from_blocked(x: Tensor, channels: int) -> Tensor:
