@@ -337,7 +337,8 @@ bool few_down(const sr355_ffn_args *a) {
 }
 
 // Small blocks of the 16-bit types, whose launches are their starts: h is held in two parts, so that y is rounded once.  The second
-// part takes 0.1 to 0.4 us there (16 x 64 x 256: down 3.3 against 3.0 us; 16 x 256 x 1024, beyond: 5.5 against 4.5).
+// part takes 0.1 to 0.4 us there (16 x 64 x 256: down 3.3 against 3.0 us; 16 x 256 x 1024, beyond: 5.5 against 4.5); larger calls
+// would pay half of the down product again.  So a row's y may differ by a step between calls of different sizes.
 bool low_kept(const sr355_ffn_args *a) {
     return a->rows <= FEW_ROWS && a->dtype != SR355_DTYPE_F32 && a->rows * a->channels * a->hidden <= (1 << 19);
 }

@@ -19,7 +19,7 @@ namespace {
 constexpr int LN_THREADS = 256;
 constexpr int LN_MAX_PARTS = 512;      // two workgroups per CU
 constexpr int LN_MOST = INT_MAX - 255; // channels: a thread's index steps by 256 behind the last one
-constexpr int LN_LONG = 8192;          // channels from which on no type's row fits a workgroup's registers
+constexpr int LN_LONG = 8192;          // channels from which on no type's row is held in registers (fp32 rows of whole units: 4096)
 
 // Partial rows of dw and db, at most: rows beyond the registers have columns enough to fill the chip with fewer.
 int ln_max_parts(int C) { return C <= LN_LONG ? LN_MAX_PARTS : C <= 65536 ? 64 : 8; }

@@ -61,9 +61,15 @@ def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, b_gate: O
               b_up: Optional[Tensor] = None, b_down: Optional[Tensor] = None, activation: str = "silu") -> Tensor:
     """``(act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down`` for rows ``x`` ``[..., C]``, ``w_gate`` and
     ``w_up`` ``[F, C]`` and ``w_down`` ``[C, F]`` (``nn.Linear`` weights), all of x's type.  ``activation``: "silu", "gelu"
-    (by the error function), "relu" or "sigmoid".  Products accumulate in fp32; the hidden channels are held in x's type
-    between the launches.  A call that autograd records keeps eight bytes (float32: twelve) per
-    hidden channel of every row of x."""
+    (by the error function), "relu" or "sigmoid".  A call that autograd records keeps eight bytes (float32: twelve) per
+    hidden channel of every row of x.
+
+    Products accumulate in fp32.  bfloat16 and float16 are rounded at these places beside the results: the hidden channels,
+    once, between the two products (y is off by some 1.4 of one rounding); the gradients of the two projections, as operands of the
+    products behind them (their bias gradients are summed before); act and the up projection times act', which the backward pass
+    reads, are cut to 24 bits.  Calls of up to 64 rows whose rows * C * F is at most 2^19 hold the hidden channels with twice their
+    bits, so y is rounded once there, and the same row may come out a step apart in a larger call; w_down's gradient takes them
+    rounded in either case."""
     if activation not in ops.ACTIVATIONS:
         raise RuntimeError(f"gated_ffn: activation must be one of {', '.join(ops.ACTIVATIONS)}, got {activation!r}")
     if not torch.compiler.is_dynamo_compiling():
