@@ -152,23 +152,19 @@ void check_capture(const std::vector<Tensor> &inputs) {
 // Whether somebody has to see the call as an operator and not as the work it does: a tensor subclass (a fake one has no memory) or
 // a dispatch mode.  The public functions then return nothing, and their caller takes the registered op.  Functional transforms are
 // refused: through a registered op a tangent would be lost.
-bool interposed(const char *who, const std::vector<Tensor> &ts) {
+template <typename... Ts>
+bool interposed(const char *who, const Ts &...ts) {
     TORCH_CHECK(!c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode), who,
                 ": functional transforms (torch.func, vmap) are not supported");
-    if (c10::impl::TorchDispatchModeTLS::any_modes_set()) return true;
-    for (const Tensor &t : ts)
-        if (t.defined() && t.key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::Functionalize}))) return true;
-    return false;
+    constexpr c10::DispatchKeySet keys({c10::DispatchKey::Python, c10::DispatchKey::Functionalize});
+    return c10::impl::TorchDispatchModeTLS::any_modes_set() || ((ts.defined() && ts.key_set().has_any(keys)) || ...);
 }
 // whether autograd records a call with these inputs
-bool recorded(const std::vector<Tensor> &ts) {
-    if (!at::GradMode::is_enabled()) return false;
-    for (const Tensor &t : ts)
-        if (t.defined() && t.requires_grad()) {
-            check_capture(ts);
-            return true;
-        }
-    return false;
+template <typename... Ts>
+bool recorded(const Ts &...ts) {
+    if (!at::GradMode::is_enabled() || !((ts.defined() && ts.requires_grad()) || ...)) return false;
+    check_capture({ts...});
+    return true;
 }
 Tensor defined(const OptTensor &t) { return t.has_value() ? *t : Tensor(); }
 
@@ -275,8 +271,8 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 Tensor layer_norm(const Tensor &x, const OptTensor &weight, const OptTensor &bias, double eps) {
     const Tensor w = defined(weight), b = defined(bias);
-    if (interposed("layer_norm", {x, w, b})) return Tensor();
-    if (recorded({x, w, b})) return LayerNorm::apply(x, weight, bias, eps);
+    if (interposed("layer_norm", x, w, b)) return Tensor();
+    if (recorded(x, w, b)) return LayerNorm::apply(x, weight, bias, eps);
     return std::get<0>(layer_norm_fwd(x, weight, bias, eps, false));
 }
 
@@ -325,8 +321,8 @@ struct Dropout : torch::autograd::Function<Dropout> {
 
 Tensor dropout(const Tensor &x, double p, const Tensor &rng, int64_t site, const OptTensor &residual) {
     const Tensor s = defined(residual);
-    if (interposed("dropout", {x, rng, s})) return Tensor();
-    if (recorded({x, s})) return Dropout::apply(x, p, rng, site, residual);
+    if (interposed("dropout", x, rng, s)) return Tensor();
+    if (recorded(x, s)) return Dropout::apply(x, p, rng, site, residual);
     return dropout_fwd(x, residual, p, rng, site);
 }
 
@@ -439,8 +435,8 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
 Tensor gated_ffn(const Tensor &x, const Tensor &w_gate, const Tensor &w_up, const Tensor &w_down, const OptTensor &b_gate,
                  const OptTensor &b_up, const OptTensor &b_down, int64_t activation) {
     const Tensor bg = defined(b_gate), bu = defined(b_up), bd = defined(b_down);
-    if (interposed("gated_ffn", {x, w_gate, w_up, w_down, bg, bu, bd})) return Tensor();
-    if (recorded({x, w_gate, w_up, w_down, bg, bu, bd}))
+    if (interposed("gated_ffn", x, w_gate, w_up, w_down, bg, bu, bd)) return Tensor();
+    if (recorded(x, w_gate, w_up, w_down, bg, bu, bd))
         return GatedFfn::apply(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation);
     return std::get<0>(gated_ffn_fwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation, false));
 }

@@ -18,6 +18,7 @@ from typing import Optional
 import torch
 import torch.distributed as dist
 from torch import Tensor, nn
+from torch.compiler import is_dynamo_compiling
 
 from . import token_ops as ops
 
@@ -33,7 +34,7 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension of ``x``.  ``weight`` and ``bias``, ``[C]``,
     are of x's type or float32 (both of one type), and so are their gradients.  A row of one channel or of equal channels
     gives ``bias`` (for ``eps`` > 0)."""
-    if not torch.compiler.is_dynamo_compiling():
+    if not is_dynamo_compiling():
         y = (ops._binding or ops.binding()).layer_norm(x, weight, bias, eps)
         if y is not None:
             return y
@@ -50,7 +51,7 @@ def dropout(x: Tensor, p: float, rng: Tensor, site: int = 0, residual: Optional[
     it runs, so a captured graph's replays drop what the words say then; changing them in place between a call and its
     backward pass is an error that autograd reports.  ``p`` counts in steps of 2^-16 and the scale is that of the nearest
     step; a dropped infinity or NaN is dropped."""
-    if not torch.compiler.is_dynamo_compiling():
+    if not is_dynamo_compiling():
         y = (ops._binding or ops.binding()).dropout(x, p, rng, site, residual)
         if y is not None:
             return y
@@ -72,7 +73,7 @@ def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, b_gate: O
     rounded in either case."""
     if activation not in ops.ACTIVATIONS:
         raise RuntimeError(f"gated_ffn: activation must be one of {', '.join(ops.ACTIVATIONS)}, got {activation!r}")
-    if not torch.compiler.is_dynamo_compiling():
+    if not is_dynamo_compiling():
         y = (ops._binding or ops.binding()).gated_ffn(x, w_gate, w_up, w_down, b_gate, b_up, b_down, ops.ACTIVATIONS[activation])
         if y is not None:
             return y
