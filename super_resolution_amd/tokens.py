@@ -33,7 +33,8 @@ def _recorded(*tensors: Optional[Tensor]) -> bool:
 def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5) -> Tensor:
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension of ``x``.  ``weight`` and ``bias``, ``[C]``,
     are of x's type or float32 (both of one type), and so are their gradients.  A row of one channel or of equal channels
-    gives ``bias`` (for ``eps`` > 0)."""
+    gives ``bias`` (for ``eps`` > 0).  Statistics and sums are float32; the backward pass takes each row's mean rounded to it, so
+    the gradients of float32 rows whose mean is some 10^4 times their deviation or more lose bits that ``y`` keeps."""
     if not is_dynamo_compiling():
         y = (ops._binding or ops.binding()).layer_norm(x, weight, bias, eps)
         if y is not None:
